@@ -36,10 +36,13 @@ extern "C" {
 /* element types of q/k/v/out */
 #define MINFER_ATTN_F16  0
 #define MINFER_ATTN_BF16 1
+#define MINFER_ATTN_F32  2  /* norm weights only */
 
 /* KV-cache formats (kv_format / cache_format fields) */
 #define MINFER_ATTN_KV_16BIT 0  /* the same 16-bit type as q                                    */
 #define MINFER_ATTN_KV_Q8_0  1  /* GGML Q8_0 blocks: 32 int8 + one fp16 scale = 34 bytes        */
+#define MINFER_ATTN_KV_E4M3  2  /* e4m3 codes, an fp32 scale per block of tokens and head (the *_b8 and norm_rope entries only) */
+#define MINFER_ATTN_KV_INT8  3  /* int8 codes, likewise                                         */
 
 /* status[0] values a kernel may leave in a caller-provided status word (device int32[4]) */
 #define MINFER_ATTN_STATUS_WAIT_TIMEOUT 100  /* {code, blockIdx.x, blockIdx.y, wait site}                       */
@@ -319,6 +322,155 @@ typedef struct MinferRopeParams {
 } MinferRopeParams;
 
 int minfer_attn_rope_append(const MinferRopeParams* params, void* stream);
+
+/*
+ * KV cache held in 8 bits ("b8"): codes [batch, n_kv_heads, max_len, head_dim], or a pool of pages
+ * [n_pages, n_kv_heads, page_size, head_dim] behind a block table, and one fp32 scale for each block of block_size
+ * consecutive rows of one head: [batch, n_kv_heads, ceil(max_len / block_size)], or [n_pages, n_kv_heads, page_size / block_size].
+ * A cached value is code * scale.  Codes are e4m3 (no infinities; 448 is the largest) or int8 (-127 .. 127);
+ * block_size is 16, 32, 64 or 128 and divides page_size; head_dim is 64 or 128.  The reference has no such cache.
+ *
+ * Code strides are in bytes (= elements), innermost 1, the others multiples of 16; bases 16-byte aligned.  Scale strides are in
+ * elements for the two outer dimensions; a head's scales are adjacent.  k and v share all strides.
+ */
+
+/*
+ * RMS norms of q's and k's heads, then rotary position embedding, then (with caches) the KV-cache append, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   over the head_dim values of every head, in fp32;
+ *   pairs of y rotated by position * freq_base^(-2 i / rotary_dim), the angle exact for any position, and rounded once.
+ * q [batch, seq, n_heads, head_dim] is rewritten in place; k and v [batch, seq, n_kv_heads, head_dim] go to cache rows
+ * start[b] + l (k normed and rotated), or without caches k is rewritten in place and v is not touched.  Any of q / k / v may be NULL
+ * (k and v together with caches).  Strides as for MinferRopeParams (elements, multiples of 8, innermost 1; pointers 16-byte aligned).
+ *
+ * q_weight / k_weight: [head_dim] (weight_stride 0) or a row per head, float16, bfloat16 or float32 (weight_dtype);
+ * 16-byte aligned, strides multiples of 16 bytes.  Both NULL: no norms.  head_dim is a multiple of 16 up to 256,
+ * rotary_dim a multiple of 8 (16 for the neox style).
+ *
+ * cache_format 16BIT: rows of the 16-bit type (cache_stride in elements, multiples of 8).  E4M3 / INT8: a b8 cache (above).
+ *   - The scale of a block follows the largest magnitude of its rows: e4m3 the smallest power of two under which it is at most
+ *     448, int8 that magnitude / 127; never below 2^-126, and 0 for a block of zeros.  Codes are nearest, ties to even.  Infinite
+ *     values saturate (and count as the largest finite one), NaN becomes e4m3's NaN or the int8 code 0.
+ *   - A block whose first row is written by this call takes its scale afresh.  A block that holds rows already (start[b] is not a
+ *     multiple of block_size) keeps them: its scale grows when the new rows need it, and then the rows before
+ *     start[b] are coded again from the values that they stood for.  It never shrinks.  Rows behind the last new one are not touched.
+ * Positions outside [0, max_len) are not written (q is still rewritten) and reported through `status`, as are entries of the
+ * block table outside [0, n_pages).  The caller sees to it that no two sequences append to the same page.
+ */
+typedef struct MinferNormRopeParams {
+  void*          q;
+  const void*    k;
+  const void*    v;
+  const void*    q_weight;
+  const void*    k_weight;
+  void*          k_cache;
+  void*          v_cache;
+  float*         k_scale;        /* b8 caches */
+  float*         v_scale;
+  const int32_t* start;          /* device int32[batch], or NULL: start_pos */
+  const int32_t* block_table;    /* NULL, or device int32[batch, table_stride] */
+  int32_t*       status;         /* optional device int32[4] */
+  int64_t q_stride[3];           /* batch, token, head */
+  int64_t kv_stride[3];
+  int64_t cache_stride[3];       /* batch (or page), head, row */
+  int64_t scale_stride[2];       /* batch (or page), head */
+  int64_t weight_stride[2];      /* q, k: elements from one head's row of weights to the next, 0: one row for all */
+  double  freq_base;
+  float   eps;
+  int32_t batch;                 /* batch * seq must stay below 2^31 - 64 */
+  int32_t seq;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t start_pos;
+  int32_t max_len;               /* rows per sequence of the caches */
+  int32_t dtype;                 /* of q, k, v and 16-bit caches */
+  int32_t weight_dtype;          /* MINFER_ATTN_F16 / _BF16 / _F32 */
+  int32_t style;                 /* 0 interleaved pairs, 1 neox */
+  int32_t cache_format;
+  int32_t block_size;            /* b8 caches */
+  int32_t page_size;
+  int32_t table_stride;
+  int32_t n_pages;
+  int32_t flags;                 /* reserved, must be 0 */
+} MinferNormRopeParams;
+
+int minfer_attn_norm_rope_append(const MinferNormRopeParams* params, void* stream);
+
+/*
+ * Decode attention (one query token per sequence) over a b8 cache; q, out, lens, softmax_scale, block_table and status as in
+ * MinferAttnDecodeParams.  Rows at lens[b] and behind, and their scales, are never read.  lens[b] == 0 yields zeros; a NaN among
+ * the visible values reaches the outputs that it enters.
+ * workspace: minfer_attn_decode_b8_workspace_bytes() bytes, 16-byte aligned, any content; 0 for most shapes.  Without it
+ * a shape that would use it takes another form (slower; the sums are split differently).
+ */
+typedef struct MinferAttnDecodeB8Params {
+  const void*    q;
+  const void*    k_cache;
+  const void*    v_cache;
+  const float*   k_scale;
+  const float*   v_scale;
+  const int32_t* lens;
+  void*          out;
+  const int32_t* block_table;
+  int32_t*       status;
+  void*          workspace;
+  size_t         workspace_bytes;
+  int64_t q_stride[2];           /* elements: batch, head */
+  int64_t kv_stride[3];          /* bytes: batch (or page), head, row */
+  int64_t scale_stride[2];       /* elements: batch (or page), head */
+  int64_t out_stride[2];
+  int32_t batch;
+  int32_t n_heads;
+  int32_t n_kv_heads;
+  int32_t max_len;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t cache_format;          /* MINFER_ATTN_KV_E4M3 or _INT8 */
+  int32_t block_size;
+  int32_t page_size;
+  int32_t table_stride;
+  int32_t n_pages;
+  int32_t flags;                 /* reserved, must be 0 */
+  float   softmax_scale;
+} MinferAttnDecodeB8Params;
+
+int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* params, void* stream);
+size_t minfer_attn_decode_b8_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t max_len, int32_t head_dim);
+
+/*
+ * Rows of a b8 cache as 16-bit values (code * scale, rounded once): row j of sequence b to row j of k_out / v_out
+ * [batch, n_kv_heads, out_rows, head_dim] for j < min(lens[b], max_len, out_rows); the other rows of the outputs are not touched.  For the
+ * attention of a prompt behind a cached prefix (minfer_attn_prefill reads 16-bit keys and values).
+ */
+typedef struct MinferKvReadB8Params {
+  const void*    k_cache;
+  const void*    v_cache;
+  const float*   k_scale;
+  const float*   v_scale;
+  const int32_t* lens;
+  const int32_t* block_table;
+  void*          k_out;
+  void*          v_out;
+  int32_t*       status;
+  int64_t cache_stride[3];       /* bytes: batch (or page), head, row */
+  int64_t scale_stride[2];
+  int64_t out_stride[3];         /* elements: batch, head, row; shared by k_out and v_out */
+  int32_t batch;
+  int32_t n_kv_heads;
+  int32_t max_len;
+  int32_t out_rows;
+  int32_t head_dim;
+  int32_t dtype;                 /* of the outputs */
+  int32_t cache_format;
+  int32_t block_size;
+  int32_t page_size;
+  int32_t table_stride;
+  int32_t n_pages;
+  int32_t flags;                 /* reserved, must be 0 */
+} MinferKvReadB8Params;
+
+int minfer_attn_kv_read_b8(const MinferKvReadB8Params* params, void* stream);
 
 const char* minfer_attn_strerror(int code);
 /* Text of the CUDA error behind the calling thread's latest MINFER_ATTN_ECUDA

@@ -22,8 +22,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT_DIR = os.path.join(HERE, "minfer", "kernels", "torch_ext")
 LIB_NAME = "libminfer_attn.so"
 SOURCES = ["attn_api.cu", "prefill_persist_sm100.cu", "mask_classify.cu", "decode_sm100.cu", "decode_static_sm100.cu",
-           "rope_append_sm100.cu"]
-HEADERS = ["attn_internal.h", "ptx.cuh"]
+           "rope_append_sm100.cu", "norm_rope_sm100.cu", "decode_b8_sm100.cu", "kv_read_sm100.cu"]
+HEADERS = ["attn_internal.h", "ptx.cuh", "decode_common.cuh", "b8.cuh"]
 # the LibTorch stable-ABI registration unit (schemas + CUDA impls that call the C ABI), host code only
 BINDING_NAME = "_C.abi3.so"
 BINDING_SOURCES = ["torch_binding/reg.cpp", "torch_binding/reg_cuda.cpp"]

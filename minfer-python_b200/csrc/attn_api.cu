@@ -184,6 +184,55 @@ int decode_parts(int64_t batch, int64_t n_kv_heads, int64_t max_len, int64_t row
   return parts;
 }
 
+// ---- block-scaled 8-bit caches ----
+bool is_b8(int32_t format) { return format == MINFER_ATTN_KV_E4M3 || format == MINFER_ATTN_KV_INT8; }
+
+// log2 of a valid number of tokens per block, or -1
+int32_t b8_log_block(int32_t block_size) {
+  return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : block_size == 128 ? 7 : -1;
+}
+
+// strides of codes (bytes) and scales (elements)
+bool b8_strides_ok(const int64_t cache[3], const int64_t scale[2]) {
+  for (int i = 0; i < 3; ++i)
+    if (cache[i] < 0 || cache[i] % 16 != 0) return false;
+  return scale[0] >= 0 && scale[1] >= 0;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// block_size > 0: pages have to hold whole blocks
+bool table_ok(const int32_t* table, int32_t page_size, int32_t table_stride, int32_t n_pages, int32_t max_len, int32_t block_size) {
+  if (table == nullptr) return true;
+  if (page_size <= 0 || table_stride <= 0 || n_pages <= 0 || !aligned4(table)) return false;
+  if (block_size > 0 && page_size % block_size != 0) return false;
+  return static_cast<int64_t>(page_size) * table_stride >= max_len;
+}
+
+// Blocks (one cluster) per (sequence, kv head) of a decode call over a b8 cache.
+int decode_b8_parts(int64_t batch, int64_t n_kv_heads, int64_t max_len, int64_t head_dim) {
+  const int64_t pairs = batch * n_kv_heads;
+  const int64_t wave = 2 * 148;
+  int parts = 1;
+  while (parts < 16 && max_len >= 64 * parts * 2) {
+    const int next = parts * 2;
+    const int64_t block_bytes = max_len / next * head_dim;
+    const int64_t limit = block_bytes >= (512 << 10) ? wave * 7 / 2 : block_bytes >= (256 << 10) ? wave * 2 : wave;
+    if (pairs * next > limit) break;
+    if (next == 16 && pairs > 12) break;
+    parts = next;
+  }
+  return parts;
+}
+
+// Keys per block of the form that leaves partial outputs in the workspace, 0 where clusters are used.
+int32_t decode_b8_chunk(int64_t batch, int64_t n_kv_heads, int64_t max_len) {
+  (void)batch;
+  (void)n_kv_heads;
+  (void)max_len;
+  return 0;
+}
+
 }  // namespace
 
 int cuda_result(cudaError_t e) {
@@ -488,6 +537,209 @@ int minfer_attn_decode(const MinferAttnDecodeParams* p, void* stream) {
 
   cudaError_t e = launch_decode(a, p->head_dim, p->dtype == MINFER_ATTN_BF16, q8, static_cast<cudaStream_t>(stream));
   return cuda_result(e);
+}
+
+int minfer_attn_norm_rope_append(const MinferNormRopeParams* p, void* stream) {
+  if (p == nullptr) return MINFER_ATTN_EINVAL;
+  if (p->q == nullptr && p->k == nullptr) return MINFER_ATTN_EINVAL;
+  if (p->batch <= 0 || p->seq <= 0 || p->head_dim <= 0 || p->head_dim % 16 != 0) return MINFER_ATTN_EINVAL;
+  if (p->head_dim > 256) return MINFER_ATTN_EUNSUPPORTED;
+  if (static_cast<int64_t>(p->batch) * p->seq >= (1ll << 31) - 64) return MINFER_ATTN_EINVAL;  // tokens are indexed in 32 bits
+  if (p->dtype != MINFER_ATTN_F16 && p->dtype != MINFER_ATTN_BF16) return MINFER_ATTN_EINVAL;
+  if (p->style != 0 && p->style != 1) return MINFER_ATTN_EINVAL;
+  if (p->rotary_dim < 0 || p->rotary_dim > p->head_dim || p->rotary_dim % (p->style == 1 ? 16 : 8) != 0) return MINFER_ATTN_EINVAL;
+  if (!(p->freq_base > 0.0) || !(p->freq_base < 1e300)) return MINFER_ATTN_EINVAL;
+  if (p->q != nullptr && (p->n_heads <= 0 || !aligned16(p->q) || !strides_ok(p->q_stride, 3))) return MINFER_ATTN_EINVAL;
+  if (p->k != nullptr && (p->n_kv_heads <= 0 || !aligned16(p->k) || !strides_ok(p->kv_stride, 3))) return MINFER_ATTN_EINVAL;
+  if (p->n_heads > 65535 || p->n_kv_heads > 65535) return MINFER_ATTN_EUNSUPPORTED;
+  // norms: of both or of neither (of what the call has)
+  const bool norm = p->q_weight != nullptr || p->k_weight != nullptr;
+  if (norm) {
+    if ((p->q != nullptr && p->q_weight == nullptr) || (p->k != nullptr && p->k_weight == nullptr)) return MINFER_ATTN_EINVAL;
+    if (p->weight_dtype != MINFER_ATTN_F16 && p->weight_dtype != MINFER_ATTN_BF16 && p->weight_dtype != MINFER_ATTN_F32) return MINFER_ATTN_EINVAL;
+    const int per16 = p->weight_dtype == MINFER_ATTN_F32 ? 4 : 8;
+    for (int i = 0; i < 2; ++i)
+      if (p->weight_stride[i] < 0 || p->weight_stride[i] % per16 != 0) return MINFER_ATTN_EINVAL;
+    if (!aligned16(p->q_weight) || !aligned16(p->k_weight)) return MINFER_ATTN_EINVAL;
+    if (!(p->eps >= 0.f)) return MINFER_ATTN_EINVAL;
+  }
+  if ((p->k_cache == nullptr) != (p->v_cache == nullptr)) return MINFER_ATTN_EINVAL;
+  const bool b8 = is_b8(p->cache_format);
+  if (p->cache_format != MINFER_ATTN_KV_16BIT && !b8) return MINFER_ATTN_EINVAL;
+  if (p->k_cache != nullptr) {
+    if (p->k == nullptr || p->v == nullptr || !aligned16(p->v) || !aligned16(p->k_cache) || !aligned16(p->v_cache)) return MINFER_ATTN_EINVAL;
+    if (p->max_len <= 0) return MINFER_ATTN_EINVAL;
+    if (p->start == nullptr && (p->start_pos < 0 || static_cast<int64_t>(p->start_pos) + p->seq > p->max_len)) return MINFER_ATTN_EINVAL;
+    if (b8) {
+      if (p->head_dim != 64 && p->head_dim != 128) return MINFER_ATTN_EUNSUPPORTED;
+      if (b8_log_block(p->block_size) < 0 || p->k_scale == nullptr || p->v_scale == nullptr || !aligned4(p->k_scale) || !aligned4(p->v_scale) ||
+          !b8_strides_ok(p->cache_stride, p->scale_stride))
+        return MINFER_ATTN_EINVAL;
+    } else if (!strides_ok(p->cache_stride, 3)) {
+      return MINFER_ATTN_EINVAL;
+    }
+    if (!table_ok(p->block_table, p->page_size, p->table_stride, p->n_pages, p->max_len, b8 ? p->block_size : 0)) return MINFER_ATTN_EINVAL;
+  } else if (p->block_table != nullptr || b8) {
+    return MINFER_ATTN_EINVAL;
+  }
+  if (p->start == nullptr && (p->start_pos < 0 || static_cast<int64_t>(p->start_pos) + p->seq > 0x7FFFFFFFll)) return MINFER_ATTN_EINVAL;
+  if (p->start != nullptr && !aligned4(p->start)) return MINFER_ATTN_EINVAL;
+  if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
+  if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
+  int rc = check_device();
+  if (rc != MINFER_ATTN_OK) return rc;
+  NormRopeArgs a{};
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->k_cache != nullptr ? p->v : nullptr;
+  a.q_weight = norm ? (p->q_weight != nullptr ? p->q_weight : p->k_weight) : nullptr;  // (one of them alone: for the one tensor that there is)
+  a.k_weight = norm ? (p->k_weight != nullptr ? p->k_weight : p->q_weight) : nullptr;
+  a.k_cache = p->k_cache;
+  a.v_cache = p->v_cache;
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.start = p->start;
+  a.block_table = p->block_table;
+  a.status = p->status;
+  for (int i = 0; i < 3; ++i) {
+    a.q_stride[i] = p->q_stride[i];
+    a.kv_stride[i] = p->kv_stride[i];
+    a.cache_stride[i] = p->cache_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    a.scale_stride[i] = p->scale_stride[i];
+    a.w_stride[i] = p->weight_stride[i];
+  }
+  a.w_kind = p->weight_dtype == MINFER_ATTN_F32 ? 2 : p->weight_dtype == MINFER_ATTN_BF16 ? 1 : 0;
+  a.batch = p->batch;
+  a.seq = p->seq;
+  a.n_heads = p->n_heads;
+  a.n_kv_heads = p->n_kv_heads;
+  a.head_dim = p->head_dim;
+  a.rotary_dim = p->rotary_dim;
+  a.start_pos = p->start_pos;
+  a.max_len = p->max_len;
+  a.page_size = p->block_table != nullptr ? p->page_size : 0;
+  a.table_stride = p->block_table != nullptr ? p->table_stride : 0;
+  a.n_pages = p->block_table != nullptr ? p->n_pages : 0;
+  a.log_block = b8 ? b8_log_block(p->block_size) : 0;
+  a.eps = p->eps;
+  return cuda_result(launch_norm_rope(a, p->dtype == MINFER_ATTN_BF16, p->style == 1, p->cache_format, p->freq_base, static_cast<cudaStream_t>(stream)));
+}
+
+size_t minfer_attn_decode_b8_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t max_len, int32_t head_dim) {
+  if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_len <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  const int32_t chunk = decode_b8_chunk(batch, n_kv_heads, max_len);
+  if (chunk == 0) return 0;
+  return static_cast<size_t>(batch) * n_heads * ((static_cast<size_t>(max_len) + chunk - 1) / chunk) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
+}
+
+int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* p, void* stream) {
+  if (p == nullptr || p->q == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->k_scale == nullptr || p->v_scale == nullptr ||
+      p->lens == nullptr || p->out == nullptr)
+    return MINFER_ATTN_EINVAL;
+  if (p->batch <= 0 || p->n_heads <= 0 || p->n_kv_heads <= 0 || p->max_len <= 0) return MINFER_ATTN_EINVAL;
+  if (p->n_heads % p->n_kv_heads != 0) return MINFER_ATTN_EINVAL;
+  if (p->dtype != MINFER_ATTN_F16 && p->dtype != MINFER_ATTN_BF16) return MINFER_ATTN_EINVAL;
+  if (!is_b8(p->cache_format)) return MINFER_ATTN_EINVAL;
+  if (p->head_dim != 64 && p->head_dim != 128) return MINFER_ATTN_EUNSUPPORTED;
+  const int group = p->n_heads / p->n_kv_heads;
+  if (group > 16) return MINFER_ATTN_EUNSUPPORTED;
+  if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->out)) return MINFER_ATTN_EINVAL;
+  if (!aligned4(p->k_scale) || !aligned4(p->v_scale) || !aligned4(p->lens)) return MINFER_ATTN_EINVAL;
+  if (!strides_ok(p->q_stride, 2) || !strides_ok(p->out_stride, 2) || !b8_strides_ok(p->kv_stride, p->scale_stride)) return MINFER_ATTN_EINVAL;
+  if (b8_log_block(p->block_size) < 0) return MINFER_ATTN_EINVAL;
+  if (!(p->softmax_scale >= 0.f)) return MINFER_ATTN_EINVAL;
+  if (p->batch > 65535 || p->n_kv_heads > 65535) return MINFER_ATTN_EUNSUPPORTED;
+  if (!table_ok(p->block_table, p->page_size, p->table_stride, p->n_pages, p->max_len, p->block_size)) return MINFER_ATTN_EINVAL;
+  if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
+  if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
+  const size_t need = minfer_attn_decode_b8_workspace_bytes(p->batch, p->n_heads, p->n_kv_heads, p->max_len, p->head_dim);
+  if (p->workspace != nullptr && need > 0 && (p->workspace_bytes < need || !aligned16(p->workspace))) return MINFER_ATTN_EWORKSPACE;
+  int rc = check_device();
+  if (rc != MINFER_ATTN_OK) return rc;
+
+  DecodeB8Args a{};
+  a.q = p->q;
+  a.k = p->k_cache;
+  a.v = p->v_cache;
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.lens = p->lens;
+  a.out = p->out;
+  a.batch = p->batch;
+  a.n_heads = p->n_heads;
+  a.n_kv_heads = p->n_kv_heads;
+  a.max_len = p->max_len;
+  a.group = group;
+  const int64_t pairs = static_cast<int64_t>(p->batch) * p->n_kv_heads;
+  if (need > 0 && p->workspace != nullptr) {
+    a.chunk = decode_b8_chunk(p->batch, p->n_kv_heads, p->max_len);
+    a.n_split = (p->max_len + a.chunk - 1) / a.chunk;
+    a.part_o = static_cast<float*>(p->workspace);
+    a.part_ml = a.part_o + static_cast<size_t>(p->batch) * p->n_heads * a.n_split * p->head_dim;
+  } else {
+    a.n_split = decode_b8_parts(p->batch, p->n_kv_heads, p->max_len, p->head_dim);
+    a.by_length = (p->batch > 1 && p->batch <= 256 && pairs * a.n_split > 2 * 148 && decode_is_large(pairs, p->max_len, p->head_dim)) ? 1 : 0;
+  }
+  for (int i = 0; i < 2; ++i) {
+    a.q_stride[i] = p->q_stride[i];
+    a.out_stride[i] = p->out_stride[i];
+    a.scale_stride[i] = p->scale_stride[i];
+  }
+  for (int i = 0; i < 3; ++i) a.kv_stride[i] = p->kv_stride[i];
+  const float scale = p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / std::sqrt(static_cast<float>(p->head_dim));
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.block_table = p->block_table;
+  a.page_size = p->block_table != nullptr ? p->page_size : 0;
+  a.table_stride = p->block_table != nullptr ? p->table_stride : 0;
+  a.n_pages = p->block_table != nullptr ? p->n_pages : 0;
+  a.status = p->status;
+  a.log_block = b8_log_block(p->block_size);
+  return cuda_result(launch_decode_b8(a, p->head_dim, p->dtype == MINFER_ATTN_BF16, p->cache_format == MINFER_ATTN_KV_INT8, static_cast<cudaStream_t>(stream)));
+}
+
+int minfer_attn_kv_read_b8(const MinferKvReadB8Params* p, void* stream) {
+  if (p == nullptr || p->k_cache == nullptr || p->v_cache == nullptr || p->k_scale == nullptr || p->v_scale == nullptr || p->lens == nullptr ||
+      p->k_out == nullptr || p->v_out == nullptr)
+    return MINFER_ATTN_EINVAL;
+  if (p->batch <= 0 || p->n_kv_heads <= 0 || p->max_len <= 0 || p->out_rows <= 0) return MINFER_ATTN_EINVAL;
+  if (p->dtype != MINFER_ATTN_F16 && p->dtype != MINFER_ATTN_BF16) return MINFER_ATTN_EINVAL;
+  if (!is_b8(p->cache_format) || b8_log_block(p->block_size) < 0) return MINFER_ATTN_EINVAL;
+  if (p->head_dim != 64 && p->head_dim != 128) return MINFER_ATTN_EUNSUPPORTED;
+  if (!aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->k_out) || !aligned16(p->v_out)) return MINFER_ATTN_EINVAL;
+  if (!aligned4(p->k_scale) || !aligned4(p->v_scale) || !aligned4(p->lens)) return MINFER_ATTN_EINVAL;
+  if (!strides_ok(p->out_stride, 3) || !b8_strides_ok(p->cache_stride, p->scale_stride)) return MINFER_ATTN_EINVAL;
+  // (sequence, head, 64 rows) triples are indexed in 32 bits
+  if ((static_cast<int64_t>(std::min(p->max_len, p->out_rows)) / 64 + 1) * p->batch * p->n_kv_heads >= (1ll << 31)) return MINFER_ATTN_EINVAL;
+  if (!table_ok(p->block_table, p->page_size, p->table_stride, p->n_pages, p->max_len, p->block_size)) return MINFER_ATTN_EINVAL;
+  if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
+  if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
+  int rc = check_device();
+  if (rc != MINFER_ATTN_OK) return rc;
+  KvReadArgs a{};
+  a.k_cache = p->k_cache;
+  a.v_cache = p->v_cache;
+  a.k_scale = p->k_scale;
+  a.v_scale = p->v_scale;
+  a.lens = p->lens;
+  a.block_table = p->block_table;
+  a.k_out = p->k_out;
+  a.v_out = p->v_out;
+  a.status = p->status;
+  for (int i = 0; i < 3; ++i) {
+    a.cache_stride[i] = p->cache_stride[i];
+    a.out_stride[i] = p->out_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) a.scale_stride[i] = p->scale_stride[i];
+  a.batch = p->batch;
+  a.n_kv_heads = p->n_kv_heads;
+  a.max_len = std::min(p->max_len, p->out_rows);
+  a.page_size = p->block_table != nullptr ? p->page_size : 0;
+  a.table_stride = p->block_table != nullptr ? p->table_stride : 0;
+  a.n_pages = p->block_table != nullptr ? p->n_pages : 0;
+  a.log_block = b8_log_block(p->block_size);
+  return cuda_result(launch_kv_read_b8(a, p->head_dim, p->dtype == MINFER_ATTN_BF16, p->cache_format == MINFER_ATTN_KV_INT8, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -129,4 +129,65 @@ struct DecodeArgs {
 
 cudaError_t launch_decode(const DecodeArgs& a, int head_dim, bool bf16, bool q8, cudaStream_t stream);
 
+// Kernel-side view of a decode call over a block-scaled 8-bit cache: kv_stride counts bytes.
+struct DecodeB8Args : DecodeArgs {
+  const float* k_scale;     // [batch or page, n_kv_heads, blocks], blocks adjacent
+  const float* v_scale;
+  int64_t scale_stride[2];  // elements: batch (or page), head
+  int32_t log_block;        // log2 of the tokens per block
+};
+
+cudaError_t launch_decode_b8(const DecodeB8Args& a, int head_dim, bool bf16, bool int8, cudaStream_t stream);
+
+// Kernel-side view of a norm + RoPE call, with or without an append.  Strides in elements (8-bit caches: bytes).
+struct NormRopeArgs {
+  void* q;                  // [batch, seq, n_heads, head_dim], in place; may be null
+  const void* k;            // [batch, seq, n_kv_heads, head_dim]; in place without caches
+  const void* v;            // null without caches
+  const void* q_weight;     // null: no norms
+  const void* k_weight;
+  void* k_cache;            // [batch or page, n_kv_heads, rows, head_dim]; null: k in place
+  void* v_cache;
+  float* k_scale;           // 8-bit caches: [batch or page, n_kv_heads, blocks]
+  float* v_scale;
+  const int32_t* start;
+  const int32_t* block_table;
+  int32_t* status;
+  int64_t q_stride[3], kv_stride[3], cache_stride[3], scale_stride[2];
+  int64_t w_stride[2];      // weights: elements from one head's row to the next (q, k), 0: one row for all heads
+  int32_t w_kind;           // 0 float16, 1 bfloat16, 2 float32
+  int32_t batch, seq, n_heads, n_kv_heads, head_dim, rotary_dim, start_pos, max_len;
+  int32_t page_size, table_stride, n_pages;
+  int32_t log_block;
+  float eps;
+  // set by the launcher
+  float inv_dim;
+  int32_t log_tb;           // tokens per block of rows, log2
+  int32_t n_touch;          // blocks of tokens that a sequence's new rows can touch
+  int32_t slices;           // thread blocks per (sequence, block of tokens) of k, and of v
+  uint64_t turns[128];      // frequencies: turns per position, as fractions of 2^64
+};
+// cache_format: MINFER_ATTN_KV_16BIT, _E4M3 or _INT8
+cudaError_t launch_norm_rope(const NormRopeArgs& a, bool bf16, bool neox, int cache_format, double freq_base, cudaStream_t stream);
+
+// Kernel-side view of a read-back of a block-scaled 8-bit cache.
+struct KvReadArgs {
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* lens;
+  const int32_t* block_table;
+  void* k_out;              // [batch, n_kv_heads, rows, head_dim] 16-bit
+  void* v_out;
+  int32_t* status;
+  int64_t cache_stride[3];  // bytes
+  int64_t scale_stride[2];
+  int64_t out_stride[3];    // elements
+  int32_t batch, n_kv_heads;
+  int32_t max_len;          // rows that both the cache and the output have
+  int32_t page_size, table_stride, n_pages, log_block;
+};
+cudaError_t launch_kv_read_b8(const KvReadArgs& a, int head_dim, bool bf16, bool int8, cudaStream_t stream);
+
 }  // namespace minfer_attn

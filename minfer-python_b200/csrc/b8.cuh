@@ -1,0 +1,152 @@
+// Values of a block-scaled 8-bit KV cache: e4m3 or int8 codes, one fp32 scale for each block of tokens and head.
+//
+//   e4m3  scale = the smallest power of two under which the block's largest magnitude is at most 448.  A floating code loses nothing to
+//         a coarse scale but the last factor of two of its range, and in exchange x / scale is exact, and rows coded
+//         again under a larger scale keep their values (unless they fall below the smallest normal code, 2^-6).
+//   int8  scale = fp32(largest magnitude / 127): a fixed step, where a power of two would cost up to a bit.
+//   code  = the one nearest to x / scale, ties to even.  Infinite values saturate; NaN stays NaN in e4m3 and becomes 0 in int8.
+// A block of zeros has scale 0 and codes 0; no other scale is below 2^-126.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace minfer_attn {
+
+constexpr int kE4M3 = 1;
+constexpr int kInt8 = 2;
+
+// the scale that a block with this largest magnitude needs
+template <int kFmt>
+__device__ __forceinline__ float b8_scale(float amax) {
+  amax = fminf(amax, 3.402823466e38f);  // an infinite value counts as the largest finite one
+  if constexpr (kFmt == kE4M3) {
+    // 448 = 1.75 * 2^8: the sum carries into the exponent when the significand is above 1.75
+    const int e = static_cast<int>((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 8;
+    return amax > 0.f ? __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23) : 0.f;
+  } else {
+    return amax > 0.f ? fmaxf(__fdiv_rn(amax, 127.f), 1.17549435e-38f) : 0.f;  // (normal, so that its inverse is finite)
+  }
+}
+
+// 1 / scale (exact for a power of two), 0 for a block of zeros
+__device__ __forceinline__ float b8_inverse(float s) { return s > 0.f ? __frcp_rn(s) : 0.f; }
+
+// the int8 code nearest to x / s: the product with 1 / s decides unless it lies within its error of a border
+__device__ __forceinline__ uint32_t int8_code(float x, float s, float r) {
+  float t = x * r;
+  t = t == t ? fminf(fmaxf(t, -127.f), 127.f) : 0.f;
+  float k = __fadd_rn(t, 12582912.f);
+  if (fabsf(fabsf(t - __fadd_rn(k, -12582912.f)) - 0.5f) < 6e-5f && s > 0.f) {
+    const float q = __fdiv_rn(x, s);
+    const float n = rintf(q);
+    k = n;
+    if (fabsf(q - n) == 0.5f) {  // a border as far as fp32 can tell: the remainder's sign says on which side
+      const float rem = fmaf(-q, s, x);
+      const bool up = s > 0.f ? rem > 0.f : rem < 0.f;
+      if (rem != 0.f) k = up ? ceilf(q) : floorf(q);
+    }
+    k = __fadd_rn(fminf(fmaxf(k, -127.f), 127.f), 12582912.f);
+  }
+  return __float_as_uint(k) & 0xFFu;
+}
+
+// two fp32 -> two e4m3 in the low 16 bits (lo in the low byte), saturating
+__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// two e4m3 (low 16 bits) -> two fp16, exact
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t pair) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(pair)));
+  return r;
+}
+
+// two int8 of a word whose bytes were XORed with 0x80 -> two fp16, exact: the byte dropped into the mantissa of 1024.0 reads
+// 1024 + 128 + q.  kSel picks the bytes of the low and high value.
+template <uint32_t kSel>
+__device__ __forceinline__ uint32_t int8_to_half2(uint32_t src) {
+  const uint32_t x = __byte_perm(src, 0x64646464u, kSel);
+  const uint32_t bias = 0x64806480u;  // 1152.0 twice
+  const __half2 q = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
+  return *reinterpret_cast<const uint32_t*>(&q);
+}
+
+// eight values -> eight codes
+template <int kFmt>
+__device__ __forceinline__ uint2 b8_code8(const float* x, float s, float r) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float* y = x + 4 * i;
+    if constexpr (kFmt == kE4M3) {
+      w[i] = e4m3_pair(y[0] * r, y[1] * r) | (e4m3_pair(y[2] * r, y[3] * r) << 16);
+    } else {
+      w[i] = int8_code(y[0], s, r) | (int8_code(y[1], s, r) << 8) | (int8_code(y[2], s, r) << 16) | (int8_code(y[3], s, r) << 24);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// eight codes -> fp32, unscaled
+template <int kFmt>
+__device__ __forceinline__ void b8_values8(uint2 c, float* x) {
+  const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t h[2];
+    if constexpr (kFmt == kE4M3) {
+      h[0] = e4m3_to_half2(w[i]);
+      h[1] = e4m3_to_half2(w[i] >> 16);
+    } else {
+      const uint32_t u = w[i] ^ 0x80808080u;
+      h[0] = int8_to_half2<0x4140>(u);
+      h[1] = int8_to_half2<0x4342>(u);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+      x[4 * i + 2 * j] = f.x;
+      x[4 * i + 2 * j + 1] = f.y;
+    }
+  }
+}
+
+// eight codes under scale s0 -> the codes of the same values under s1
+template <int kFmt>
+__device__ __forceinline__ uint2 b8_recode8(uint2 c, float s0, float s1, float r1) {
+  float x[8];
+  b8_values8<kFmt>(c, x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= s0;
+  return b8_code8<kFmt>(x, s1, r1);
+}
+
+// rows [0, n) of a block (row_chunks 16-byte chunks each), coded again by `lanes` threads
+template <int kFmt>
+__device__ __forceinline__ void recode_rows(uint8_t* rows, int64_t row_stride, int n, int row_chunks, float s0, float s1, int lane, int lanes) {
+  const float r1 = b8_inverse(s1);
+  constexpr int kBatch = 4;  // loads in flight
+  for (int i0 = lane; i0 < n * row_chunks; i0 += kBatch * lanes) {
+    uint4 c[kBatch];
+    uint4* p[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * lanes;
+      p[u] = i < n * row_chunks ? reinterpret_cast<uint4*>(rows + static_cast<int64_t>(i / row_chunks) * row_stride) + i % row_chunks : nullptr;
+      c[u] = p[u] != nullptr ? *p[u] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (p[u] == nullptr) continue;
+      const uint2 lo = b8_recode8<kFmt>(make_uint2(c[u].x, c[u].y), s0, s1, r1);
+      const uint2 hi = b8_recode8<kFmt>(make_uint2(c[u].z, c[u].w), s0, s1, r1);
+      *p[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  }
+}
+
+}  // namespace minfer_attn

@@ -1,0 +1,436 @@
+// Split-KV decode attention over a cache held in 8 bits (e4m3 or int8 codes) with one fp32 scale for each block of tokens and
+// head, HBM-bound: 2 head_dim + 8 / block bytes per cached key.
+//
+//   t_j = (q . k_j) ks_j / sqrt(head_dim)      out = sum_j exp(t_j) vs_j v_j / sum_j exp(t_j)
+//
+// k_j, v_j: codes; ks_j, vs_j: the scales of key j's block.  The scheme is decode_kernel's (decode_sm100.cu): a block streams a
+// part of the keys of one (sequence, kv head) for all its query heads, each warp with a ring of 16-key tiles of its own;
+// products transposed (keys, then dimensions, as the 16 rows of an m16n8k16 tile); partial outputs merged through the
+// shared memory of a cluster, or through a workspace (decode_common.cuh).  What differs:
+//
+// A tile lies inside one block of tokens, so its two scales are uniform and neither costs a multiplication per value: ks goes
+// into the factor that the scores take anyway, vs into the weights.  Codes of both kinds are exact in fp16, so all products are
+// fp16 MMAs on unscaled codes; bfloat16 queries are brought into fp16's range by a power of two per head (exact but for
+// elements below 2^-39 of the head's largest).
+//
+// Weights: w_j = 2^(t_j - m) vs_j is what is rounded to fp16.  m follows max_j(t_j + ceil(log2 vs_j)) - 14, not max t_j, so that
+// whatever the scales are the largest weight lies in (2^13, 2^14]: fp16 has full precision down to 2^-14, so weights keep theirs down to
+// 2^-28 of the largest, and a long tail of equal small weights is not rounded in one direction.  The row sum takes 2^(t_j - m)
+// in fp32, before the scale and before the rounding.  log2 vs_j counts as -90 or more: 2^104 times the number of keys fits
+// fp32, and a block of zeros (scale 0) has weights of 0.
+//
+// Shared memory: rows of 128 bytes with the 16-byte chunks XORed by the row, pairs of rows of 64 bytes likewise by their line, so that a lane's
+// 16-byte reads - K: chunks 2 tq and 2 tq + 1 of key g0; V: chunk g0 of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 - meet no bank twice.
+// A lane takes consecutive dimensions: for K that permutes the summands of an MMA, for V the rows of the output.
+#include "b8.cuh"
+#include "decode_common.cuh"
+
+#include <atomic>
+
+namespace minfer_attn {
+
+namespace {
+
+#ifndef MINFER_ATTN_B8_STAGES
+#define MINFER_ATTN_B8_STAGES 6
+#endif
+#ifndef MINFER_ATTN_B8_CTAS
+#define MINFER_ATTN_B8_CTAS 2
+#endif
+constexpr float kWeightLog = 14.f;   // log2 of the largest weight, as stored
+constexpr int kLeastScaleLog = -90;  // a scale's log2, as far as the reference m follows it
+
+template <int D, int NT>
+struct LayoutB8 {
+  static constexpr int kStages = MINFER_ATTN_B8_STAGES;
+  static constexpr int kTileBytes = kTileKeys * D;
+  static constexpr int kStageBytes = 2 * kTileBytes + 16;  // K, V, the tile's scales (two floats)
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kRingBytes = kWarps * kWarpBytes;
+  static constexpr int kWmlBytes = kWarps * 8 * NT * 8;
+  static constexpr int kPartBytes = 8 * NT * D * 4;
+  static constexpr int kMlBytes = kMaxParts * 8 * NT * 8;
+  static constexpr int kBytes = kRingBytes + kWmlBytes + kPartBytes + kMlBytes + 16;  // + the arrival barrier, an abort flag
+  static_assert(kWarpBytes >= 8 * NT * (D + 4) * 4, "the per-warp ring also holds the warp's partial output");
+  static_assert(kRingBytes >= (kMaxRanked + 2) * 4, "the ranking by length borrows the ring");
+};
+
+// byte offset of a 16-byte chunk of a row inside a tile
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+  if constexpr (D == 128) return row * 128 + ((chunk ^ (row & 7)) << 4);
+  const int line = row >> 1;
+  return line * 128 + (((((row & 1) << 2) | chunk) ^ ((line & 3) << 1)) << 4);
+}
+
+__device__ __forceinline__ void cp_async_4(void* smem_dst, const void* gsrc) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(gsrc) : "memory");
+}
+
+// four codes of a word -> two pairs of fp16: the A fragments of keys (K), or of one key pair's two dimensions (V, kHigh picks them)
+template <bool I8>
+__device__ __forceinline__ void word_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (I8) {
+    const uint32_t u = w ^ 0x80808080u;
+    lo = int8_to_half2<0x4140>(u);
+    hi = int8_to_half2<0x4342>(u);
+  } else {
+    lo = e4m3_to_half2(w);
+    hi = e4m3_to_half2(w >> 16);
+  }
+}
+
+template <int D, bool BF16, bool I8, bool Paged, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? MINFER_ATTN_B8_CTAS : 2) decode_b8_kernel(const DecodeB8Args a) {
+  using L = LayoutB8<D, NT>;
+  constexpr int kSt = L::kStages;
+  constexpr int kTileBytes = L::kTileBytes;
+  constexpr int kWarpBytes = L::kWarpBytes;
+  constexpr int kChunksPerRow = D / 16;
+  constexpr int kRowsPerLoad = 32 / kChunksPerRow;           // rows that one instruction of a warp brings
+  constexpr int kLoads = kTileKeys / kRowsPerLoad;
+
+  extern __shared__ __align__(128) uint8_t smem[];
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int kvh = blockIdx.y;
+  const bool clustered = a.part_o == nullptr;
+  const int part = blockIdx.x;
+  const int n_parts = gridDim.x;
+
+  uint64_t* arrived = reinterpret_cast<uint64_t*>(smem + L::kBytes - 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(arrived + 1);
+  grid_launch_dependents();
+  if (clustered && n_parts > 1) {
+    if (tid == 0) {
+      *abort_flag = 0;
+      mbar_init(arrived, 1);
+      mbar_fence_init();
+      mbar_arrive_expect_tx(arrived, static_cast<uint32_t>(a.group * (D * 4 + n_parts * 8)));
+    }
+    __syncwarp();
+    cluster_arrive();
+  }
+  grid_dependency_wait();
+
+  int b = blockIdx.z, len;
+  if (a.by_length) {
+    const int2 x = sequence_by_length(a.lens, a.batch, a.max_len, b, reinterpret_cast<int*>(smem), tid);
+    b = x.x;
+    len = x.y;
+  } else {
+    len = max(0, min(a.lens[b], a.max_len));
+  }
+  int c0, c1;
+  if (clustered) {
+    const int nt_seq = (len + kTileKeys - 1) / kTileKeys;
+    c0 = static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part) / static_cast<unsigned>(n_parts)) * kTileKeys;
+    c1 = min(len, static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part + 1) / static_cast<unsigned>(n_parts)) * kTileKeys);
+  } else {
+    c0 = part * a.chunk;
+    if (c0 >= len) return;
+    c1 = min(len, c0 + a.chunk);
+  }
+  const int nt = c1 > c0 ? (c1 - c0 + kTileKeys - 1) / kTileKeys : 0;
+  const int nt_w = (nt > warp) ? (nt - warp + kWarps - 1) / kWarps : 0;
+
+  uint8_t* wsm = smem + warp * kWarpBytes;
+  const int l_row = lane / kChunksPerRow, l_chunk = lane % kChunksPerRow;
+
+  auto issue_tile = [&](int i) {  // i-th tile of this warp -> stage i % kSt
+    if (i < nt_w) {
+      const int key0 = c0 + (warp + i * kWarps) * kTileKeys;
+      int64_t toff = static_cast<int64_t>(kvh) * a.kv_stride[1];
+      int64_t soff = static_cast<int64_t>(kvh) * a.scale_stride[1];
+      if constexpr (Paged) {
+        const int slot = key0 / a.page_size;
+        int page = a.block_table[static_cast<size_t>(b) * a.table_stride + slot];
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.n_pages)) {
+          if (lane == 0) report_bad_page(a.status, b, slot, page);
+          page = 0;
+        }
+        const int row = key0 - slot * a.page_size;
+        toff += static_cast<int64_t>(page) * a.kv_stride[0] + static_cast<int64_t>(row) * a.kv_stride[2];
+        soff += static_cast<int64_t>(page) * a.scale_stride[0] + (row >> a.log_block);
+      } else {
+        toff += static_cast<int64_t>(b) * a.kv_stride[0] + static_cast<int64_t>(key0) * a.kv_stride[2];
+        soff += static_cast<int64_t>(b) * a.scale_stride[0] + (key0 >> a.log_block);
+      }
+      uint8_t* dst_k = wsm + (i % kSt) * L::kStageBytes;
+      uint8_t* dst_v = dst_k + kTileBytes;
+      const uint8_t* src_k = reinterpret_cast<const uint8_t*>(a.k) + toff + l_chunk * 16;
+      const uint8_t* src_v = reinterpret_cast<const uint8_t*>(a.v) + toff + l_chunk * 16;
+      const int live = c1 - key0;
+#pragma unroll
+      for (int t = 0; t < kLoads; ++t) {
+        const int row = t * kRowsPerLoad + l_row;
+        const bool pred = row < live;  // rows beyond the sequence are not read and count as zeros
+        const int64_t off = static_cast<int64_t>(pred ? row : 0) * a.kv_stride[2];
+        const uint32_t at = chunk_at<D>(row, l_chunk);
+        cp_async_16(dst_k + at, src_k + off, pred);
+        cp_async_16(dst_v + at, src_v + off, pred);
+      }
+      if (lane < 2) cp_async_4(dst_k + 2 * kTileBytes + 4 * lane, (lane == 0 ? a.k_scale : a.v_scale) + soff);
+    }
+    cp_async_commit();
+  };
+
+  if (a.by_length) __syncthreads();  // the ranking's scratch is the ring's memory
+#pragma unroll
+  for (int s = 0; s < kSt - 1; ++s) issue_tile(s);
+
+  // ---- Q^T fragments (B operand), fp16: step (u, i) holds dimensions 16 (2 tq + u) + 4 i + {0 .. 3} of lane tq (head_dim 64: 16 tq + 4 i) ----
+  const int g0 = lane >> 2;
+  const int tq = lane & 3;
+  constexpr int kU = D / 64;
+  uint32_t qf[NT][D / 16][2];
+  float qs[NT][2];  // per column (heads 2 tq, 2 tq + 1): softmax scale * log2(e) * the power of two taken out of the queries
+  {
+    const uint8_t* qb = reinterpret_cast<const uint8_t*>(a.q) + 2 * static_cast<int64_t>(b) * a.q_stride[0];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int g = g0 + 8 * n;
+      const bool live = g < a.group;
+      const uint8_t* qp = qb + 2 * static_cast<int64_t>(kvh * a.group + (live ? g : 0)) * a.q_stride[1];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 x = *reinterpret_cast<const uint4*>(qp + 32 * (kU * tq + u) + 16 * h);
+          qf[n][4 * u + 2 * h][0] = live ? x.x : 0u;
+          qf[n][4 * u + 2 * h][1] = live ? x.y : 0u;
+          qf[n][4 * u + 2 * h + 1][0] = live ? x.z : 0u;
+          qf[n][4 * u + 2 * h + 1][1] = live ? x.w : 0u;
+        }
+      }
+      float back = 1.f;  // of head g
+      if constexpr (BF16) {
+        uint32_t top = 0;  // largest magnitude, as bits
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) top = max(top, max(qf[n][s][e] & 0x7FFFu, (qf[n][s][e] >> 16) & 0x7FFFu));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        // the largest becomes 2^14 .. 2^15; exponents kept so that neither factor leaves fp32's range
+        const int e = max(-110, min(110, 127 + 14 - static_cast<int>(top >> 7)));
+        const float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        back = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+            qf[n][s][w] = pack2<false>(__uint_as_float(qf[n][s][w] << 16) * f, __uint_as_float(qf[n][s][w] & 0xFFFF0000u) * f);
+      }
+      qs[n][0] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq);
+      qs[n][1] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq + 4);
+    }
+  }
+
+  float oacc[NT][D / 16][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) oacc[n][m][0] = oacc[n][m][1] = oacc[n][m][2] = oacc[n][m][3] = 0.f;
+  float m_ref[NT][2], l_run[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m_ref[n][0] = m_ref[n][1] = -INFINITY;
+    l_run[n][0] = l_run[n][1] = 0.f;
+  }
+
+  for (int i = 0; i < nt_w; ++i) {
+    cp_async_wait<kSt - 2>();
+    __syncwarp();
+    issue_tile(i + kSt - 1);
+
+    const int key0 = c0 + (warp + i * kWarps) * kTileKeys;
+    const uint8_t* tk = wsm + (i % kSt) * L::kStageBytes;
+    const uint8_t* tv = tk + kTileBytes;
+    const float2 scales = *reinterpret_cast<const float2*>(tk + 2 * kTileBytes);
+    // ---- S^T[16 keys x 8 heads] = K Q^T (two accumulators: half the chain of dependent MMAs) ----
+    float s[NT][4], s2[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint4 x = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0, kU * tq + u));
+      const uint4 y = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0 + 8, kU * tq + u));
+      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t kf[4];
+        word_to_half<I8>(xw[w], kf[0], kf[2]);
+        word_to_half<I8>(yw[w], kf[1], kf[3]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_16816<false>((w & 1) ? s2[n] : s[n], kf, qf[n][4 * u + w][0], qf[n][4 * u + w][1]);
+      }
+    }
+    // ---- online softmax: x = t - m; 2^x times the scale has to stay within 2^14; a tile in which it does needs no reduction over
+    // the lanes ----
+    const bool partial = key0 + kTileKeys > c1;
+    const bool dead0 = partial && key0 + g0 >= c1, dead1 = partial && key0 + g0 + 8 >= c1;
+    const float room = kWeightLog - static_cast<float>(max(static_cast<int>((__float_as_uint(scales.y) + 0x7FFFFFu) >> 23) - 127, kLeastScaleLog));
+    float x[NT][4];
+    bool move = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float f0 = qs[n][0] * scales.x, f1 = qs[n][1] * scales.x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = (s[n][e] + s2[n][e]) * ((e & 1) ? f1 : f0);
+        if (e < 2 ? dead0 : dead1) s[n][e] = -INFINITY;
+        x[n][e] = s[n][e] - m_ref[n][e & 1];  // +inf before the first tile (-inf - -inf: NaN, which moves nothing)
+      }
+      move |= fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) > room;
+    }
+    if (__any_sync(0xFFFFFFFFu, move)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float alpha[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(s[n][h], s[n][2 + h]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+          const float m_new = fmaxf(m_ref[n][h], mx - room);
+          alpha[h] = ex2_approx(m_ref[n][h] - m_new);
+          m_ref[n][h] = m_new;
+          l_run[n][h] *= alpha[h];
+        }
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) {
+          oacc[n][m][0] *= alpha[0];
+          oacc[n][m][1] *= alpha[1];
+          oacc[n][m][2] *= alpha[0];
+          oacc[n][m][3] *= alpha[1];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = s[n][e] - m_ref[n][e & 1];
+      }
+    }
+    uint32_t pb[NT][2];  // P^T fragments (B operand): keys 2 tq, 2 tq + 1 (+ 8) of head g0
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] = ex2_approx(x[n][e]);
+      l_run[n][0] += x[n][0] + x[n][2];
+      l_run[n][1] += x[n][1] + x[n][3];
+      pb[n][0] = movmatrix_trans(pack2<false>(x[n][0] * scales.y, x[n][1] * scales.y));
+      pb[n][1] = movmatrix_trans(pack2<false>(x[n][2] * scales.y, x[n][3] * scales.y));
+    }
+
+    // ---- O^T[D x 8 heads] += V^T P^T: lane (g0, tq) reads D / 8 dimensions of its four keys and interleaves the keys pairwise; rows g0 and
+    // g0 + 8 of 16-row tile m are dimensions (D / 8) g0 + 2 m and + 1 ----
+    constexpr int kVWords = D / 32;
+    uint32_t vw[4][kVWords];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 2 * tq + (r & 1) + 8 * (r >> 1);
+      if constexpr (D == 128) {
+        const uint4 y = *reinterpret_cast<const uint4*>(tv + chunk_at<D>(row, g0));
+        vw[r][0] = y.x;
+        vw[r][1] = y.y;
+        vw[r][2] = y.z;
+        vw[r][3] = y.w;
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(tv + chunk_at<D>(row, g0 >> 1) + 8 * (g0 & 1));
+        vw[r][0] = y.x;
+        vw[r][1] = y.y;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) {
+      const int w = m >> 1;
+      uint32_t vf[4];
+      word_to_half<I8>(__byte_perm(vw[0][w], vw[1][w], (m & 1) ? 0x7362 : 0x5140), vf[0], vf[1]);
+      word_to_half<I8>(__byte_perm(vw[2][w], vw[3][w], (m & 1) ? 0x7362 : 0x5140), vf[2], vf[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_16816<false>(oacc[n][m], vf, pb[n][0], pb[n][1]);
+    }
+  }
+  cp_async_wait<0>();
+
+  // ---- this warp's partial output into its part of the ring ----
+  const int group = a.group;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 4);
+      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 8);
+      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 16);
+    }
+  __syncthreads();
+  constexpr int kRow = D + 4;
+  float* mo = reinterpret_cast<float*>(wsm);
+  float2* wml = reinterpret_cast<float2*>(smem + L::kRingBytes);
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int g = 8 * n + 2 * tq + h;
+      if (g < group) {
+#pragma unroll
+        for (int m = 0; m < D / 16; m += 2)
+          *reinterpret_cast<float4*>(&mo[g * kRow + (D / 8) * g0 + 2 * m]) =
+              make_float4(oacc[n][m][h], oacc[n][m][2 + h], oacc[n][m + 1][h], oacc[n][m + 1][2 + h]);
+        if (g0 == 0) wml[warp * 8 * NT + g] = make_float2(m_ref[n][h], l_run[n][h]);
+      }
+    }
+  merge_partials<D, BF16, NT, L, true>(a, smem, arrived, abort_flag, b, kvh, part, n_parts, clustered, tid);
+}
+
+template <int D, bool BF16, bool I8, bool Paged, int NT>
+cudaError_t launch_heads(const DecodeB8Args& a, cudaStream_t stream) {
+  auto* kernel = decode_b8_kernel<D, BF16, I8, Paged, NT>;
+  constexpr int smem = LayoutB8<D, NT>::kBytes;
+  static std::atomic<bool> attr_done[64] = {};  // set-once flags; the attribute calls themselves are idempotent
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
+  }
+  const bool clustered = a.part_o == nullptr;
+  LaunchAttrs at(stream);
+  at.cfg.gridDim = dim3(a.n_split, a.n_kv_heads, a.batch);
+  at.cfg.blockDim = dim3(kWarps * 32);
+  at.cfg.dynamicSmemBytes = smem;
+  if (clustered && a.n_split > 1) at.cluster(a.n_split);
+  e = cudaLaunchKernelEx(&at.cfg, kernel, a);
+  if (e != cudaSuccess || clustered) return e;
+  LaunchAttrs ac(stream);
+  ac.cfg.gridDim = dim3(a.n_heads, a.batch);
+  ac.cfg.blockDim = dim3(D);
+  return cudaLaunchKernelEx(&ac.cfg, decode_combine_kernel<D, BF16, true>, static_cast<const DecodeArgs&>(a));
+}
+
+template <int D, bool BF16, bool I8>
+cudaError_t launch_one(const DecodeB8Args& a, cudaStream_t stream) {
+  if (a.group <= 8)
+    return a.block_table != nullptr ? launch_heads<D, BF16, I8, true, 1>(a, stream) : launch_heads<D, BF16, I8, false, 1>(a, stream);
+  return a.block_table != nullptr ? launch_heads<D, BF16, I8, true, 2>(a, stream) : launch_heads<D, BF16, I8, false, 2>(a, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_decode_b8(const DecodeB8Args& a, int head_dim, bool bf16, bool int8, cudaStream_t stream) {
+  if (int8) {
+    if (head_dim == 128) return bf16 ? launch_one<128, true, true>(a, stream) : launch_one<128, false, true>(a, stream);
+    return bf16 ? launch_one<64, true, true>(a, stream) : launch_one<64, false, true>(a, stream);
+  }
+  if (head_dim == 128) return bf16 ? launch_one<128, true, false>(a, stream) : launch_one<128, false, false>(a, stream);
+  return bf16 ? launch_one<64, true, false>(a, stream) : launch_one<64, false, false>(a, stream);
+}
+
+}  // namespace minfer_attn

@@ -10,6 +10,7 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/ops/empty.h>
 #include <ATen/record_function.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -44,6 +45,12 @@ struct DirectEnv {
     return e.s;
   }
   static int max_ctas() { return binding_max_ctas(); }
+  struct Guard {  // (calls on another device than the current one are not served here)
+    explicit Guard(const Tensor&) {}
+  };
+  static Tensor temporary(const Tensor& like, size_t bytes) {
+    return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+  }
   template <class P>
   static int call(int (*fn)(const P*, void*), const P* p, void* stream) {
     // a launch waits while the stream's queue is full: other Python threads run meanwhile
@@ -170,6 +177,69 @@ PyObject* rope_kv_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return attempt(ready, [&] { Ops::rope_kv_append_paged(rot, base, style, *t[0], *t[1], *t[2], *t[3], *t[4], *t[5], *t[6]); });
 }
 
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  std::array<at::Tensor*, 5> t;
+  int64_t rot, style;
+  double base, eps;
+  const bool ready = n == 9 && thread_is_plain() && as_int(a[0], rot) && as_double(a[1], base) && as_int(a[2], style) && as_double(a[3], eps) && plain_tensors(a, 4, t);
+  return attempt(ready, [&] { Ops::qk_norm_rope(rot, base, style, eps, *t[0], *t[1], *t[2], *t[3], *t[4]); });
+}
+
+PyObject* qk_norm_rope_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  std::array<at::Tensor*, 8> t;
+  int64_t rot, style;
+  double base, eps;
+  const bool ready = n == 12 && thread_is_plain() && as_int(a[0], rot) && as_double(a[1], base) && as_int(a[2], style) && as_double(a[3], eps) && plain_tensors(a, 4, t);
+  return attempt(ready, [&] { Ops::qk_norm_rope_kv_append(rot, base, style, eps, *t[0], *t[1], *t[2], *t[3], *t[4], *t[5], *t[6], *t[7]); });
+}
+
+PyObject* qk_norm_rope_kv_append_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  std::array<at::Tensor*, 9> t;
+  int64_t rot, style;
+  double base, eps;
+  const bool ready = n == 13 && thread_is_plain() && as_int(a[0], rot) && as_double(a[1], base) && as_int(a[2], style) && as_double(a[3], eps) && plain_tensors(a, 4, t);
+  return attempt(ready, [&] { Ops::qk_norm_rope_kv_append_paged(rot, base, style, eps, *t[0], *t[1], *t[2], *t[3], *t[4], *t[5], *t[6], *t[7], *t[8]); });
+}
+
+// (rotary_dim, freq_base, style, q, k, v, caches, scales, block_size, [block_table,] start, q_weight or None, k_weight or None, eps)
+template <bool Paged>
+PyObject* rope_kv_append_b8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr int kPaged = Paged ? 1 : 0;
+  std::array<at::Tensor*, 7> t;
+  std::array<at::Tensor*, 1 + kPaged> u;
+  std::array<at::Tensor*, 2> w;
+  int64_t rot, style, block;
+  double base, eps;
+  bool ready = n == 15 + kPaged && thread_is_plain() && as_int(a[0], rot) && as_double(a[1], base) && as_int(a[2], style) && plain_tensors(a, 3, t) &&
+               as_int(a[10], block) && plain_tensors(a, 11, u) && as_double(a[14 + kPaged], eps);
+  const bool norm = ready && a[12 + kPaged] != Py_None;
+  if (ready) ready = norm ? plain_tensors(a, 12 + kPaged, w) : a[13 + kPaged] == Py_None;
+  return attempt(ready, [&] {
+    Ops::norm_rope(rot, base, style, eps, *t[0], *t[1], t[2], norm ? w[0] : nullptr, norm ? w[1] : nullptr, t[3], t[4], t[5], t[6], block,
+                   Paged ? u[0] : nullptr, *u[kPaged]);
+  });
+}
+
+template <bool Paged>
+PyObject* flash_attn_decode_b8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr int kPaged = Paged ? 1 : 0;
+  std::array<at::Tensor*, 5> t;
+  std::array<at::Tensor*, 2 + kPaged> u;
+  int64_t block;
+  const bool ready = n == 8 + kPaged && thread_is_plain() && plain_tensors(a, 0, t) && as_int(a[5], block) && plain_tensors(a, 6, u);
+  return attempt(ready, [&] { Ops::decode_b8(*t[0], *t[1], *t[2], *t[3], *t[4], block, Paged ? u[0] : nullptr, *u[kPaged], *u[1 + kPaged]); });
+}
+
+template <bool Paged>
+PyObject* kv_read_b8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr int kPaged = Paged ? 1 : 0;
+  std::array<at::Tensor*, 4> t;
+  std::array<at::Tensor*, 3 + kPaged> u;
+  int64_t block;
+  const bool ready = n == 8 + kPaged && thread_is_plain() && plain_tensors(a, 0, t) && as_int(a[4], block) && plain_tensors(a, 5, u);
+  return attempt(ready, [&] { Ops::read_b8(*t[0], *t[1], *t[2], *t[3], block, Paged ? u[0] : nullptr, *u[kPaged], *u[1 + kPaged], *u[2 + kPaged]); });
+}
+
 #define MINFER_DIRECT(name, fn) \
   { name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
@@ -183,6 +253,15 @@ PyMethodDef methods[] = {
     MINFER_DIRECT("rope_kv_append", &rope_kv_append<false>),
     MINFER_DIRECT("rope_kv_append_q8", &rope_kv_append<true>),
     MINFER_DIRECT("rope_kv_append_paged", &rope_kv_append_paged),
+    MINFER_DIRECT("qk_norm_rope", &qk_norm_rope),
+    MINFER_DIRECT("qk_norm_rope_kv_append", &qk_norm_rope_kv_append),
+    MINFER_DIRECT("qk_norm_rope_kv_append_paged", &qk_norm_rope_kv_append_paged),
+    MINFER_DIRECT("rope_kv_append_b8", &rope_kv_append_b8<false>),
+    MINFER_DIRECT("rope_kv_append_b8_paged", &rope_kv_append_b8<true>),
+    MINFER_DIRECT("flash_attn_decode_b8", &flash_attn_decode_b8<false>),
+    MINFER_DIRECT("flash_attn_decode_b8_paged", &flash_attn_decode_b8<true>),
+    MINFER_DIRECT("kv_read_b8", &kv_read_b8<false>),
+    MINFER_DIRECT("kv_read_b8_paged", &kv_read_b8<true>),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "attention ops without the dispatcher; each returns whether it served the call", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

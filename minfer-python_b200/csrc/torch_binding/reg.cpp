@@ -33,6 +33,15 @@ STABLE_TORCH_LIBRARY(minfer, m) {
   m.def("rope_kv_append(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(a!) v_cache, Tensor start) -> ()");
   m.def("rope_kv_append_q8(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(a!) v_cache, Tensor start) -> ()");
   m.def("rope_kv_append_paged(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(a!) v_pages, Tensor block_table, Tensor start) -> ()");
+  m.def("qk_norm_rope(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor(b!) k, Tensor q_weight, Tensor k_weight, Tensor start) -> ()");
+  m.def("qk_norm_rope_kv_append(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor k, Tensor v, Tensor q_weight, Tensor k_weight, Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor start) -> ()");
+  m.def("qk_norm_rope_kv_append_paged(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor k, Tensor v, Tensor q_weight, Tensor k_weight, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor block_table, Tensor start) -> ()");
+  m.def("rope_kv_append_b8(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor(d!) k_scale, Tensor(e!) v_scale, int block_size, Tensor start, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06) -> ()");
+  m.def("rope_kv_append_b8_paged(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) k_scale, Tensor(e!) v_scale, int block_size, Tensor block_table, Tensor start, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06) -> ()");
+  m.def("flash_attn_decode_b8(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int block_size, Tensor lens, Tensor(a!) out) -> ()");
+  m.def("flash_attn_decode_b8_paged(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scale, Tensor v_scale, int block_size, Tensor block_table, Tensor lens, Tensor(a!) out) -> ()");
+  m.def("kv_read_b8(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int block_size, Tensor lens, Tensor(a!) k_out, Tensor(b!) v_out) -> ()");
+  m.def("kv_read_b8_paged(Tensor k_pages, Tensor v_pages, Tensor k_scale, Tensor v_scale, int block_size, Tensor block_table, Tensor lens, Tensor(a!) k_out, Tensor(b!) v_out) -> ()");
   // housekeeping of this binding: the device's status word, and the grid limit of later prefill calls
   m.def("attn_status_word(Tensor like) -> Tensor");
   m.def("attn_set_prefill_cta_limit(Tensor like, int max_ctas) -> ()");

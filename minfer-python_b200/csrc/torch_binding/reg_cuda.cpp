@@ -119,6 +119,15 @@ struct StableEnv {
     return {t.mutable_data_ptr(), static_cast<size_t>(t.numel())};
   }
   static int max_ctas() { return g_max_ctas; }
+  // the tensor's device is the current one while this lives
+  struct Guard {
+    torch::stable::accelerator::DeviceGuard guard;
+    explicit Guard(const Tensor& t) : guard(t.get_device_index()) {}
+  };
+  static Tensor temporary(const Tensor& like, size_t bytes) {
+    const int64_t n[1] = {static_cast<int64_t>(bytes)};
+    return torch::stable::new_empty(like, {n, 1}, ScalarType::Byte);
+  }
   template <class P>
   static int call(int (*fn)(const P*, void*), const P* p, void* stream) { return fn(p, stream); }
 };
@@ -158,6 +167,15 @@ STABLE_TORCH_LIBRARY_IMPL(minfer, CUDA, m) {
   m.impl("rope_kv_append", TORCH_BOX(&Ops::rope_kv_append));
   m.impl("rope_kv_append_q8", TORCH_BOX(&Ops::rope_kv_append_q8));
   m.impl("rope_kv_append_paged", TORCH_BOX(&Ops::rope_kv_append_paged));
+  m.impl("qk_norm_rope", TORCH_BOX(&Ops::qk_norm_rope));
+  m.impl("qk_norm_rope_kv_append", TORCH_BOX(&Ops::qk_norm_rope_kv_append));
+  m.impl("qk_norm_rope_kv_append_paged", TORCH_BOX(&Ops::qk_norm_rope_kv_append_paged));
+  m.impl("rope_kv_append_b8", TORCH_BOX(&Ops::rope_kv_append_b8));
+  m.impl("rope_kv_append_b8_paged", TORCH_BOX(&Ops::rope_kv_append_b8_paged));
+  m.impl("flash_attn_decode_b8", TORCH_BOX(&Ops::flash_attn_decode_b8));
+  m.impl("flash_attn_decode_b8_paged", TORCH_BOX(&Ops::flash_attn_decode_b8_paged));
+  m.impl("kv_read_b8", TORCH_BOX(&Ops::kv_read_b8));
+  m.impl("kv_read_b8_paged", TORCH_BOX(&Ops::kv_read_b8_paged));
   m.impl("attn_status_word", TORCH_BOX(&attn_status_word_cuda));
   m.impl("attn_set_prefill_cta_limit", TORCH_BOX(&attn_set_prefill_cta_limit_cuda));
 }

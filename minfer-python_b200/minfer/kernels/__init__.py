@@ -2,7 +2,8 @@
 
 Only the attention path's attributes exist: `flash_attn`, `il_rope` and `neox_rope`
 keep the reference's signatures; `flash_attn_causal`, `flash_attn_decode` (also over a
-Q8_0 or a paged cache) and `rope_kv_append` are additions.
+Q8_0, a paged or a block-scaled 8-bit cache, "b8"), `rope_kv_append` (likewise),
+`qk_norm_rope` and `kv_read_b8` are additions.
 """
 
 
@@ -13,6 +14,18 @@ class KernelBackend:
             from .torch_ext import il_rope, neox_rope, rope_kv_append
             from .torch_ext import flash_attn_decode_q8, rope_kv_append_q8
             from .torch_ext import flash_attn_decode_paged, rope_kv_append_paged
+            from .torch_ext import qk_norm_rope, qk_norm_rope_kv_append, qk_norm_rope_kv_append_paged
+            from .torch_ext import rope_kv_append_b8, flash_attn_decode_b8, kv_read_b8
+            from .torch_ext import rope_kv_append_b8_paged, flash_attn_decode_b8_paged, kv_read_b8_paged
+            self.qk_norm_rope = qk_norm_rope
+            self.qk_norm_rope_kv_append = qk_norm_rope_kv_append
+            self.qk_norm_rope_kv_append_paged = qk_norm_rope_kv_append_paged
+            self.rope_kv_append_b8 = rope_kv_append_b8
+            self.flash_attn_decode_b8 = flash_attn_decode_b8
+            self.kv_read_b8 = kv_read_b8
+            self.rope_kv_append_b8_paged = rope_kv_append_b8_paged
+            self.flash_attn_decode_b8_paged = flash_attn_decode_b8_paged
+            self.kv_read_b8_paged = kv_read_b8_paged
             self.flash_attn_decode_paged = flash_attn_decode_paged
             self.rope_kv_append_paged = rope_kv_append_paged
             self.flash_attn_decode_q8 = flash_attn_decode_q8

@@ -11,3 +11,6 @@ from .ops import flash_attn, flash_attn_causal, flash_attn_decode  # noqa: F401
 from .ops import il_rope, neox_rope, rope_kv_append  # noqa: F401
 from .ops import flash_attn_decode_q8, rope_kv_append_q8  # noqa: F401
 from .ops import flash_attn_decode_paged, rope_kv_append_paged  # noqa: F401
+from .ops import qk_norm_rope, qk_norm_rope_kv_append, qk_norm_rope_kv_append_paged  # noqa: F401
+from .ops import rope_kv_append_b8, flash_attn_decode_b8, kv_read_b8  # noqa: F401
+from .ops import rope_kv_append_b8_paged, flash_attn_decode_b8_paged, kv_read_b8_paged  # noqa: F401

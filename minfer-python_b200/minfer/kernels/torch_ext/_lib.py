@@ -14,8 +14,11 @@ LIB_PATH = os.environ.get("MINFER_ATTN_LIBRARY") or os.path.join(_HERE, "libminf
 
 F16 = 0
 BF16 = 1
+F32 = 2  # norm weights only
 KV_16BIT = 0
 KV_Q8_0 = 1
+KV_E4M3 = 2
+KV_INT8 = 3
 ABI_VERSION = 5
 
 EXPORTS = (
@@ -27,6 +30,10 @@ EXPORTS = (
     "minfer_attn_rope_append",
     "minfer_attn_decode_workspace_bytes",
     "minfer_attn_decode_default_chunk",
+    "minfer_attn_norm_rope_append",
+    "minfer_attn_decode_b8",
+    "minfer_attn_decode_b8_workspace_bytes",
+    "minfer_attn_kv_read_b8",
     "minfer_attn_strerror",
     "minfer_attn_last_cuda_error",
     "minfer_attn_abi_version",
@@ -126,6 +133,109 @@ class RopeParams(ctypes.Structure):
     ]
 
 
+class NormRopeParams(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("start", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("kv_stride", ctypes.c_int64 * 3),
+        ("cache_stride", ctypes.c_int64 * 3),
+        ("scale_stride", ctypes.c_int64 * 2),
+        ("weight_stride", ctypes.c_int64 * 2),
+        ("freq_base", ctypes.c_double),
+        ("eps", ctypes.c_float),
+        ("batch", ctypes.c_int32),
+        ("seq", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("start_pos", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("style", ctypes.c_int32),
+        ("cache_format", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+    ]
+
+
+class DecodeB8Params(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("q_stride", ctypes.c_int64 * 2),
+        ("kv_stride", ctypes.c_int64 * 3),
+        ("scale_stride", ctypes.c_int64 * 2),
+        ("out_stride", ctypes.c_int64 * 2),
+        ("batch", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_format", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class KvReadB8Params(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("v_out", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("cache_stride", ctypes.c_int64 * 3),
+        ("scale_stride", ctypes.c_int64 * 2),
+        ("out_stride", ctypes.c_int64 * 3),
+        ("batch", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("max_len", ctypes.c_int32),
+        ("out_rows", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_format", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+    ]
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -149,6 +259,12 @@ def _load() -> ctypes.CDLL:
     lib.minfer_attn_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.minfer_attn_decode_default_chunk.argtypes = [ctypes.c_int32] * 3
     lib.minfer_attn_decode_default_chunk.restype = ctypes.c_int32
+    for name, params in (("minfer_attn_norm_rope_append", NormRopeParams), ("minfer_attn_decode_b8", DecodeB8Params),
+                         ("minfer_attn_kv_read_b8", KvReadB8Params)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.minfer_attn_decode_b8_workspace_bytes.argtypes = [ctypes.c_int32] * 5
+    lib.minfer_attn_decode_b8_workspace_bytes.restype = ctypes.c_size_t
     lib.minfer_attn_strerror.argtypes = [ctypes.c_int]
     lib.minfer_attn_strerror.restype = ctypes.c_char_p
     lib.minfer_attn_last_cuda_error.argtypes = []

@@ -74,6 +74,32 @@ _DEFS = {
                             "Tensor(a!) k_pages, Tensor(a!) v_pages, Tensor block_table, Tensor start) -> ()",
     "rope_kv_append_q8": "(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, "
                          "Tensor(a!) k_cache, Tensor(a!) v_cache, Tensor start) -> ()",
+    # norms of every q and k head, then the rotation (and the append), in one pass
+    "qk_norm_rope": "(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor(b!) k, "
+                    "Tensor q_weight, Tensor k_weight, Tensor start) -> ()",
+    "qk_norm_rope_kv_append": "(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor k, Tensor "
+                              "v, Tensor q_weight, Tensor k_weight, Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor "
+                              "start) -> ()",
+    "qk_norm_rope_kv_append_paged": "(int rotary_dim, float freq_base, int style, float eps, Tensor(a!) q, Tensor k, Tensor "
+                                    "v, Tensor q_weight, Tensor k_weight, Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor "
+                                    "block_table, Tensor start) -> ()",
+    # KV cache in 8 bits (float8_e4m3fn or int8 codes) with one fp32 scale per block of tokens and head
+    "rope_kv_append_b8": "(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, "
+                         "Tensor(b!) k_cache, Tensor(c!) v_cache, Tensor(d!) k_scale, Tensor(e!) v_scale, int "
+                         "block_size, Tensor start, Tensor? q_weight=None, Tensor? k_weight=None, float eps=1e-06) "
+                         "-> ()",
+    "rope_kv_append_b8_paged": "(int rotary_dim, float freq_base, int style, Tensor(a!) q, Tensor k, Tensor v, "
+                               "Tensor(b!) k_pages, Tensor(c!) v_pages, Tensor(d!) k_scale, Tensor(e!) v_scale, int "
+                               "block_size, Tensor block_table, Tensor start, Tensor? q_weight=None, Tensor? "
+                               "k_weight=None, float eps=1e-06) -> ()",
+    "flash_attn_decode_b8": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int "
+                            "block_size, Tensor lens, Tensor(a!) out) -> ()",
+    "flash_attn_decode_b8_paged": "(Tensor q, Tensor k_pages, Tensor v_pages, Tensor k_scale, Tensor v_scale, int "
+                                  "block_size, Tensor block_table, Tensor lens, Tensor(a!) out) -> ()",
+    "kv_read_b8": "(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int block_size, Tensor "
+                  "lens, Tensor(a!) k_out, Tensor(b!) v_out) -> ()",
+    "kv_read_b8_paged": "(Tensor k_pages, Tensor v_pages, Tensor k_scale, Tensor v_scale, int block_size, Tensor "
+                        "block_table, Tensor lens, Tensor(a!) k_out, Tensor(b!) v_out) -> ()",
 }
 _binding_choice = os.environ.get("MINFER_ATTN_BINDING", "auto")
 if _binding_choice not in ("auto", "ctypes", "stable"):
@@ -402,11 +428,215 @@ def _rope_kv_append_cuda(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache
     _rope_call(p, q.device)
 
 
+def _check_on(like, **tensors) -> None:
+    torch._check(like.is_cuda, lambda: "all tensors must be on CUDA")
+    for name, t in tensors.items():
+        torch._check(t.is_cuda and t.device == like.device, lambda name=name: f"{name} must be on the same CUDA device as the others")
+
+
+def _check_int_vector(t, like, n: int, what: str) -> None:
+    _check_on(like, **{what: t})
+    torch._check(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.numel() == n,
+                 lambda: f"{what} must be a contiguous int32 vector with one entry per sequence")
+
+
+def _check_caches(k, v, like, block_table, batch: int) -> None:
+    _check_on(like, k_cache=k, v_cache=v)
+    torch._check(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype,
+                 lambda: "the caches must be [B, Hkv, Lmax, D] (or pools [n_pages, Hkv, page_size, D]) of one type, shape and strides")
+    torch._check(k.stride(3) == 1, lambda: "innermost stride must be 1")
+    torch._check(block_table is not None or k.size(0) == batch, lambda: "batch mismatch")
+    if block_table is not None:
+        _check_on(like, block_table=block_table)
+        torch._check(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.is_contiguous() and
+                     block_table.size(0) == batch, lambda: "block_table must be a contiguous CUDA int32 [B, max_pages] tensor")
+
+
+def _b8_format(cache) -> int:
+    torch._check(cache.dtype in (torch.float8_e4m3fn, torch.int8), lambda: "8-bit caches are float8_e4m3fn or int8 tensors")
+    return _lib.KV_INT8 if cache.dtype == torch.int8 else _lib.KV_E4M3
+
+
+def _check_scales(ks, vs, cache, block_size: int) -> None:
+    _check_on(cache, k_scale=ks, v_scale=vs)
+    torch._check(block_size in (16, 32, 64, 128), lambda: "block_size must be 16, 32, 64 or 128")
+    torch._check(ks.dtype == torch.float32 and vs.dtype == torch.float32, lambda: "scales must be float32")
+    torch._check(ks.dim() == 3 and ks.shape == vs.shape and ks.stride() == vs.stride(),
+                 lambda: "the scales must be 3-D and share shape and strides")
+    torch._check(ks.size(0) == cache.size(0) and ks.size(1) == cache.size(1) and ks.size(2) == -(-cache.size(2) // block_size),
+                 lambda: "scales must be [B or n_pages, Hkv, rows / block_size (rounded up)]")
+    torch._check(ks.size(2) <= 1 or ks.stride(2) == 1, lambda: "a head's scales must be adjacent")
+
+
+def _set_table(p, cache, block_table) -> None:
+    p.max_len = cache.size(2)
+    if block_table is not None:
+        p.block_table = block_table.data_ptr()
+        p.page_size, p.table_stride, p.n_pages = cache.size(2), block_table.size(1), cache.size(0)
+        torch._check(cache.size(2) * block_table.size(1) <= 2 ** 31 - 1, lambda: "page_size * max_pages out of range")
+        p.max_len = cache.size(2) * block_table.size(1)
+
+
+def _set_b8(p, k_cache, v_cache, k_scale, v_scale, block_size) -> None:
+    p.cache_format = _b8_format(k_cache)
+    _check_scales(k_scale, v_scale, k_cache, block_size)
+    p.k_scale, p.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    p.scale_stride[0], p.scale_stride[1] = k_scale.stride(0), k_scale.stride(1)
+    p.block_size = block_size
+
+
+def _launch(fn: str, p, device) -> None:
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream().cuda_stream
+        _lib.check(getattr(_lib.lib, fn)(ctypes.byref(p), ctypes.c_void_p(stream)), fn)
+
+
+def _norm_rope(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, k_scale, v_scale, block_size,
+               block_table, start) -> None:
+    _check_on(q, k=k)
+    torch._check(q.dim() == 4 and k.dim() == 4, lambda: "q and k must be [B, L, heads, head_dim]")
+    torch._check(q.dtype == k.dtype, lambda: "dtypes differ")
+    torch._check(q.size(0) == k.size(0) and q.size(1) == k.size(1) and q.size(3) == k.size(3), lambda: "batch / seq / head_dim mismatch")
+    torch._check(q.stride(3) == 1 and k.stride(3) == 1, lambda: "innermost stride must be 1")
+    torch._check(0 <= rotary_dim <= q.size(3), lambda: "rotary_dim exceeds head_dim")
+    _check_int_vector(start, q, q.size(0), "start")
+    p = _lib.NormRopeParams()
+    p.dtype = _dtype_tag(q)
+    if v is not None:
+        _check_on(q, v=v)
+        torch._check(v.dtype == k.dtype and v.shape == k.shape and v.stride() == k.stride(), lambda: "k and v must share dtype, shape and strides")
+        _check_caches(k_cache, v_cache, q, block_table, q.size(0))
+        torch._check(k_cache.size(1) == k.size(2) and k_cache.size(3) == k.size(3), lambda: "head count / head_dim mismatch")
+        if k_scale is not None:
+            _set_b8(p, k_cache, v_cache, k_scale, v_scale, block_size)
+        else:
+            torch._check(k_cache.dtype == q.dtype, lambda: "dtypes differ")
+        _set_table(p, k_cache, block_table)
+        p.v, p.k_cache, p.v_cache = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+        for i in range(3):
+            p.cache_stride[i] = k_cache.stride(i)
+    torch._check((q_weight is None) == (k_weight is None), lambda: "q_weight and k_weight go together")
+    if q_weight is not None:
+        torch._check(q_weight.dtype == k_weight.dtype, lambda: "the weights must share one dtype")
+        p.weight_dtype = _lib.F32 if q_weight.dtype == torch.float32 else _dtype_tag(q_weight)
+        for i, (w, heads, name) in enumerate(((q_weight, q.size(2), "q_weight"), (k_weight, k.size(2), "k_weight"))):
+            _check_on(q, **{name: w})
+            torch._check(w.dim() in (1, 2) and w.size(-1) == q.size(3) and (w.dim() == 1 or w.size(0) == heads) and w.stride(-1) == 1,
+                         lambda name=name: f"{name} must be [head_dim] or [heads, head_dim] with innermost stride 1")
+            p.weight_stride[i] = w.stride(0) if w.dim() == 2 and heads > 1 else 0
+        p.q_weight, p.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
+    p.q, p.k, p.start = q.data_ptr(), k.data_ptr(), start.data_ptr()
+    for i in range(3):
+        p.q_stride[i], p.kv_stride[i] = q.stride(i), k.stride(i)
+    p.freq_base, p.eps = freq_base, eps
+    p.batch, p.seq, p.n_heads, p.n_kv_heads, p.head_dim = q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)
+    p.rotary_dim, p.style = rotary_dim, style if style in (0, 1) else -1
+    p.status = _status_word(q.device).data_ptr()
+    _launch("minfer_attn_norm_rope_append", p, q.device)
+
+
+def _qk_norm_rope_cuda(rotary_dim, freq_base, style, eps, q, k, q_weight, k_weight, start) -> None:
+    _norm_rope(rotary_dim, freq_base, style, eps, q, k, None, q_weight, k_weight, None, None, None, None, 0, None, start)
+
+
+def _qk_norm_rope_kv_append_cuda(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, start) -> None:
+    _norm_rope(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, None, None, 0, None, start)
+
+
+def _qk_norm_rope_kv_append_paged_cuda(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_pages, v_pages, block_table,
+                                       start) -> None:
+    _norm_rope(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_pages, v_pages, None, None, 0, block_table, start)
+
+
+def _rope_kv_append_b8_cuda(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, k_scale, v_scale, block_size, start,
+                            q_weight=None, k_weight=None, eps=1e-6) -> None:
+    _norm_rope(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, k_scale, v_scale, block_size, None, start)
+
+
+def _rope_kv_append_b8_paged_cuda(rotary_dim, freq_base, style, q, k, v, k_pages, v_pages, k_scale, v_scale, block_size, block_table,
+                                  start, q_weight=None, k_weight=None, eps=1e-6) -> None:
+    _norm_rope(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_pages, v_pages, k_scale, v_scale, block_size, block_table,
+               start)
+
+
+def _decode_b8(q, k_cache, v_cache, k_scale, v_scale, block_size, block_table, lens, out) -> None:
+    _check_on(q, out=out)
+    torch._check(q.dim() == 4 and out.dim() == 4 and q.shape == out.shape and q.dtype == out.dtype,
+                 lambda: "q/out must be [B, H, 1, D] tensors of one dtype")
+    torch._check(q.size(2) == 1, lambda: "decode takes one query token per sequence")
+    torch._check(q.stride(3) == 1 and out.stride(3) == 1, lambda: "innermost stride must be 1")
+    _check_caches(k_cache, v_cache, q, block_table, q.size(0))
+    torch._check(k_cache.size(3) == q.size(3) and k_cache.size(1) > 0 and q.size(1) % k_cache.size(1) == 0,
+                 lambda: "head_dim mismatch, or n_heads no multiple of n_kv_heads")
+    p = _lib.DecodeB8Params()
+    _set_b8(p, k_cache, v_cache, k_scale, v_scale, block_size)
+    _check_int_vector(lens, q, q.size(0), "lens")
+    p.q, p.k_cache, p.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    p.lens, p.out = lens.data_ptr(), out.data_ptr()
+    for i in range(2):
+        p.q_stride[i], p.out_stride[i] = q.stride(i), out.stride(i)
+    for i in range(3):
+        p.kv_stride[i] = k_cache.stride(i)
+    _set_table(p, k_cache, block_table)
+    p.batch, p.n_heads, p.n_kv_heads, p.head_dim = q.size(0), q.size(1), k_cache.size(1), q.size(3)
+    p.dtype = _dtype_tag(q)
+    p.status = _status_word(q.device).data_ptr()
+    need = _lib.lib.minfer_attn_decode_b8_workspace_bytes(p.batch, p.n_heads, p.n_kv_heads, p.max_len, p.head_dim)
+    with torch.cuda.device(q.device):
+        # a buffer of this call's own: torch's allocator keeps it apart from other streams' and other graphs' calls
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        if ws is not None:
+            p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        _launch("minfer_attn_decode_b8", p, q.device)
+
+
+def _flash_attn_decode_b8_cuda(q, k_cache, v_cache, k_scale, v_scale, block_size, lens, out) -> None:
+    _decode_b8(q, k_cache, v_cache, k_scale, v_scale, block_size, None, lens, out)
+
+
+def _flash_attn_decode_b8_paged_cuda(q, k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, out) -> None:
+    _decode_b8(q, k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, out)
+
+
+def _kv_read(k_cache, v_cache, k_scale, v_scale, block_size, block_table, lens, k_out, v_out) -> None:
+    _check_on(k_out, v_out=v_out)
+    torch._check(k_out.dim() == 4 and k_out.shape == v_out.shape and k_out.stride() == v_out.stride() and k_out.dtype == v_out.dtype and
+                 k_out.stride(3) == 1, lambda: "k_out and v_out must be [B, Hkv, rows, D] tensors of one dtype, shape and strides, innermost stride 1")
+    _check_caches(k_cache, v_cache, k_out, block_table, k_out.size(0))
+    torch._check(k_cache.size(1) == k_out.size(1) and k_cache.size(3) == k_out.size(3), lambda: "head count / head_dim mismatch")
+    p = _lib.KvReadB8Params()
+    _set_b8(p, k_cache, v_cache, k_scale, v_scale, block_size)
+    _check_int_vector(lens, k_out, k_out.size(0), "lens")
+    p.k_cache, p.v_cache, p.lens = k_cache.data_ptr(), v_cache.data_ptr(), lens.data_ptr()
+    p.k_out, p.v_out = k_out.data_ptr(), v_out.data_ptr()
+    for i in range(3):
+        p.cache_stride[i], p.out_stride[i] = k_cache.stride(i), k_out.stride(i)
+    _set_table(p, k_cache, block_table)
+    p.batch, p.n_kv_heads, p.out_rows, p.head_dim = k_out.size(0), k_out.size(1), k_out.size(2), k_out.size(3)
+    p.dtype = _dtype_tag(k_out)
+    p.status = _status_word(k_out.device).data_ptr()
+    _launch("minfer_attn_kv_read_b8", p, k_out.device)
+
+
+def _kv_read_b8_cuda(k_cache, v_cache, k_scale, v_scale, block_size, lens, k_out, v_out) -> None:
+    _kv_read(k_cache, v_cache, k_scale, v_scale, block_size, None, lens, k_out, v_out)
+
+
+def _kv_read_b8_paged_cuda(k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, k_out, v_out) -> None:
+    _kv_read(k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, k_out, v_out)
+
+
 for _name, _fn in (("il_rope", _il_rope_cuda), ("neox_rope", _neox_rope_cuda), ("rope_kv_append", _rope_kv_append_cuda),
                    ("rope_kv_append_q8", _rope_kv_append_q8_cuda), ("rope_kv_append_paged", _rope_kv_append_paged_cuda),
                    ("flash_attn_decode_q8", _flash_attn_decode_q8_cuda), ("flash_attn", _flash_attn_cuda),
                    ("flash_attn_causal", _flash_attn_causal_cuda), ("flash_attn_decode", _flash_attn_decode_cuda),
-                   ("flash_attn_decode_paged", _flash_attn_decode_paged_cuda)):
+                   ("flash_attn_decode_paged", _flash_attn_decode_paged_cuda), ("qk_norm_rope", _qk_norm_rope_cuda),
+                   ("qk_norm_rope_kv_append", _qk_norm_rope_kv_append_cuda),
+                   ("qk_norm_rope_kv_append_paged", _qk_norm_rope_kv_append_paged_cuda),
+                   ("rope_kv_append_b8", _rope_kv_append_b8_cuda), ("rope_kv_append_b8_paged", _rope_kv_append_b8_paged_cuda),
+                   ("flash_attn_decode_b8", _flash_attn_decode_b8_cuda),
+                   ("flash_attn_decode_b8_paged", _flash_attn_decode_b8_paged_cuda), ("kv_read_b8", _kv_read_b8_cuda),
+                   ("kv_read_b8_paged", _kv_read_b8_paged_cuda)):
     if _name not in _IN_EXTENSION:
         _library.impl(_name, _fn, "CUDA")
 
@@ -522,6 +752,119 @@ def rope_kv_append_q8(rotary_dim: int, freq_base: float, style: int, q: torch.Te
     return torch.ops.minfer.rope_kv_append_q8.default(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, start)
 
 
+def qk_norm_rope(rotary_dim: int, freq_base: float, style: int, eps: float, q: torch.Tensor, k: torch.Tensor,
+                 q_weight: torch.Tensor, k_weight: torch.Tensor, start: torch.Tensor):
+    """
+    RMS norm of every head of q [B, L, Hq, D] and k [B, L, Hkv, D], then the rotation by positions start[b] + l (start: int32 [B]),
+    both in place: x * rsqrt(mean(x^2) + eps) * weight in fp32, rounded once after the rotation.  Weights: [D] or
+    [heads, D], float16, bfloat16 or float32.  style 0 = interleaved (il_rope), 1 = neox; D a multiple of 16 up to 256.
+    Angles are exact for any position (rope_kv_append's are fp32 products).
+    """
+    if _direct is not None and not _is_compiling() and _direct.qk_norm_rope(rotary_dim, freq_base, style, eps, q, k, q_weight, k_weight, start):
+        return None
+    return torch.ops.minfer.qk_norm_rope.default(rotary_dim, freq_base, style, eps, q, k, q_weight, k_weight, start)
+
+
+def qk_norm_rope_kv_append(rotary_dim: int, freq_base: float, style: int, eps: float, q: torch.Tensor, k: torch.Tensor,
+                           v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, start: torch.Tensor):
+    """qk_norm_rope with k (normed and rotated) and plain v written to the caches [B, Hkv, Lmax, D] at rows start[b] + l;
+    q in place, k and v unchanged."""
+    if _direct is not None and not _is_compiling() and _direct.qk_norm_rope_kv_append(
+            rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, start):
+        return None
+    return torch.ops.minfer.qk_norm_rope_kv_append.default(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache,
+                                                           v_cache, start)
+
+
+def qk_norm_rope_kv_append_paged(rotary_dim: int, freq_base: float, style: int, eps: float, q: torch.Tensor, k: torch.Tensor,
+                                 v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, k_pages: torch.Tensor,
+                                 v_pages: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor):
+    """qk_norm_rope_kv_append into a paged cache: pools [n_pages, Hkv, page_size, D], block_table int32 [B, max_pages]."""
+    if _direct is not None and not _is_compiling() and _direct.qk_norm_rope_kv_append_paged(
+            rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_pages, v_pages, block_table, start):
+        return None
+    return torch.ops.minfer.qk_norm_rope_kv_append_paged.default(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight,
+                                                                 k_pages, v_pages, block_table, start)
+
+
+def rope_kv_append_b8(rotary_dim: int, freq_base: float, style: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_size: int,
+                      start: torch.Tensor, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                      eps: float = 1e-6):
+    """
+    the step before attention on a cache held in 8 bits: rotate q [B, L, Hq, D] in place, write rotated k and plain v [B, L, Hkv, D]
+    as codes to rows start[b] + l of the caches [B, Hkv, Lmax, D] (float8_e4m3fn or int8; D 64 or 128), with one float32
+    scale per block of block_size (16, 32, 64, 128) rows of a head: k_scale / v_scale [B, Hkv, ceil(Lmax / block_size)].
+    With q_weight and k_weight the heads are RMS-normed first (see qk_norm_rope).
+
+    A block whose first row is written here takes its scale afresh (e4m3: the smallest power of two under which the largest
+    magnitude is at most 448; int8: largest magnitude / 127).  A block that holds rows already keeps them; its scale grows when the
+    new rows need it, and the rows are then coded again.
+    """
+    if _direct is not None and not _is_compiling() and _direct.rope_kv_append_b8(
+            rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, k_scale, v_scale, block_size, start, q_weight, k_weight, eps):
+        return None
+    return torch.ops.minfer.rope_kv_append_b8.default(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, k_scale, v_scale,
+                                                      block_size, start, q_weight, k_weight, eps)
+
+
+def rope_kv_append_b8_paged(rotary_dim: int, freq_base: float, style: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                            block_size: int, block_table: torch.Tensor, start: torch.Tensor, q_weight: torch.Tensor | None = None,
+                            k_weight: torch.Tensor | None = None, eps: float = 1e-6):
+    """rope_kv_append_b8 into a paged cache: pools [n_pages, Hkv, page_size, D], scales [n_pages, Hkv, page_size / block_size],
+    block_table int32 [B, max_pages]; page_size a multiple of block_size."""
+    if _direct is not None and not _is_compiling() and _direct.rope_kv_append_b8_paged(
+            rotary_dim, freq_base, style, q, k, v, k_pages, v_pages, k_scale, v_scale, block_size, block_table, start, q_weight, k_weight,
+            eps):
+        return None
+    return torch.ops.minfer.rope_kv_append_b8_paged.default(rotary_dim, freq_base, style, q, k, v, k_pages, v_pages, k_scale, v_scale,
+                                                            block_size, block_table, start, q_weight, k_weight, eps)
+
+
+def flash_attn_decode_b8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                         block_size: int, lens: torch.Tensor, out: torch.Tensor):
+    """
+    flash_attn_decode over a cache held in 8 bits (layout: rope_kv_append_b8): q/out [B, n_heads, 1, D], lens int32 [B]; sequence b
+    attends keys [0, lens[b]), each value code * scale of its block.
+    """
+    if _direct is not None and not _is_compiling() and _direct.flash_attn_decode_b8(q, k_cache, v_cache, k_scale, v_scale, block_size, lens, out):
+        return None
+    return torch.ops.minfer.flash_attn_decode_b8.default(q, k_cache, v_cache, k_scale, v_scale, block_size, lens, out)
+
+
+def flash_attn_decode_b8_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor,
+                               v_scale: torch.Tensor, block_size: int, block_table: torch.Tensor, lens: torch.Tensor, out: torch.Tensor):
+    """flash_attn_decode_b8 over a paged cache (layout: rope_kv_append_b8_paged).  Only the table entries below
+    ceil(lens[b] / page_size) are read."""
+    if _direct is not None and not _is_compiling() and _direct.flash_attn_decode_b8_paged(
+            q, k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, out):
+        return None
+    return torch.ops.minfer.flash_attn_decode_b8_paged.default(q, k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, out)
+
+
+def kv_read_b8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_size: int,
+               lens: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor):
+    """
+    rows [0, lens[b]) of a cache held in 8 bits (layout: rope_kv_append_b8) as 16-bit values, code * scale rounded once, into k_out and
+    v_out [B, Hkv, rows, D] (float16 or bfloat16); rows of the outputs behind lens[b] are left as they are.  For
+    flash_attn_causal of a prompt behind a cached prefix.
+    """
+    if _direct is not None and not _is_compiling() and _direct.kv_read_b8(k_cache, v_cache, k_scale, v_scale, block_size, lens, k_out, v_out):
+        return None
+    return torch.ops.minfer.kv_read_b8.default(k_cache, v_cache, k_scale, v_scale, block_size, lens, k_out, v_out)
+
+
+def kv_read_b8_paged(k_pages: torch.Tensor, v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_size: int,
+                     block_table: torch.Tensor, lens: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor):
+    """kv_read_b8 over a paged cache (layout: rope_kv_append_b8_paged)."""
+    if _direct is not None and not _is_compiling() and _direct.kv_read_b8_paged(
+            k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, k_out, v_out):
+        return None
+    return torch.ops.minfer.kv_read_b8_paged.default(k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, k_out, v_out)
+
+
 @torch.library.register_fake("minfer::flash_attn_decode_q8")
 def _(q, k_cache, v_cache, lens, out):
     torch._check(q.dtype in (torch.float16, torch.bfloat16) and out.dtype == q.dtype)
@@ -545,6 +888,78 @@ def _(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, start):
     torch._check(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8)
     torch._check(start.dtype == torch.int32)
     torch._check(q.device.type == "cuda")
+
+
+def _fake_turn(q, k, start):
+    torch._check(q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype)
+    torch._check(q.dim() == 4 and k.dim() == 4)
+    torch._check(start.dtype == torch.int32)
+    torch._check(q.device.type == "cuda")
+
+
+def _fake_b8(k_cache, v_cache, k_scale, v_scale):
+    torch._check(k_cache.dtype in (torch.float8_e4m3fn, torch.int8) and v_cache.dtype == k_cache.dtype)
+    torch._check(k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32)
+    torch._check(k_cache.dim() == 4 and v_cache.dim() == 4 and k_scale.dim() == 3 and v_scale.dim() == 3)
+
+
+@torch.library.register_fake("minfer::qk_norm_rope")
+def _(rotary_dim, freq_base, style, eps, q, k, q_weight, k_weight, start):
+    _fake_turn(q, k, start)
+
+
+@torch.library.register_fake("minfer::qk_norm_rope_kv_append")
+def _(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_cache, v_cache, start):
+    _fake_turn(q, k, start)
+    torch._check(v.dtype == q.dtype and k_cache.dtype == q.dtype and v_cache.dtype == q.dtype)
+
+
+@torch.library.register_fake("minfer::qk_norm_rope_kv_append_paged")
+def _(rotary_dim, freq_base, style, eps, q, k, v, q_weight, k_weight, k_pages, v_pages, block_table, start):
+    _fake_turn(q, k, start)
+    torch._check(v.dtype == q.dtype and k_pages.dtype == q.dtype and v_pages.dtype == q.dtype and block_table.dtype == torch.int32)
+
+
+@torch.library.register_fake("minfer::rope_kv_append_b8")
+def _(rotary_dim, freq_base, style, q, k, v, k_cache, v_cache, k_scale, v_scale, block_size, start, q_weight=None, k_weight=None, eps=1e-6):
+    _fake_turn(q, k, start)
+    _fake_b8(k_cache, v_cache, k_scale, v_scale)
+
+
+@torch.library.register_fake("minfer::rope_kv_append_b8_paged")
+def _(rotary_dim, freq_base, style, q, k, v, k_pages, v_pages, k_scale, v_scale, block_size, block_table, start, q_weight=None,
+      k_weight=None, eps=1e-6):
+    _fake_turn(q, k, start)
+    _fake_b8(k_pages, v_pages, k_scale, v_scale)
+    torch._check(block_table.dtype == torch.int32)
+
+
+@torch.library.register_fake("minfer::flash_attn_decode_b8")
+def _(q, k_cache, v_cache, k_scale, v_scale, block_size, lens, out):
+    torch._check(q.dtype in (torch.float16, torch.bfloat16) and out.dtype == q.dtype and q.device.type == "cuda")
+    _fake_b8(k_cache, v_cache, k_scale, v_scale)
+    torch._check(lens.dtype == torch.int32)
+
+
+@torch.library.register_fake("minfer::flash_attn_decode_b8_paged")
+def _(q, k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, out):
+    torch._check(q.dtype in (torch.float16, torch.bfloat16) and out.dtype == q.dtype and q.device.type == "cuda")
+    _fake_b8(k_pages, v_pages, k_scale, v_scale)
+    torch._check(lens.dtype == torch.int32 and block_table.dtype == torch.int32)
+
+
+@torch.library.register_fake("minfer::kv_read_b8")
+def _(k_cache, v_cache, k_scale, v_scale, block_size, lens, k_out, v_out):
+    torch._check(k_out.dtype in (torch.float16, torch.bfloat16) and v_out.dtype == k_out.dtype and k_out.device.type == "cuda")
+    _fake_b8(k_cache, v_cache, k_scale, v_scale)
+    torch._check(lens.dtype == torch.int32)
+
+
+@torch.library.register_fake("minfer::kv_read_b8_paged")
+def _(k_pages, v_pages, k_scale, v_scale, block_size, block_table, lens, k_out, v_out):
+    torch._check(k_out.dtype in (torch.float16, torch.bfloat16) and v_out.dtype == k_out.dtype and k_out.device.type == "cuda")
+    _fake_b8(k_pages, v_pages, k_scale, v_scale)
+    torch._check(lens.dtype == torch.int32 and block_table.dtype == torch.int32)
 
 
 @torch.library.register_fake("minfer::il_rope")

@@ -300,3 +300,93 @@ def within_tolerance(actual: torch.Tensor, expected: torch.Tensor, atol: float =
     bad = err > (atol + rtol * e.abs())
     bad |= ~torch.isfinite(a)
     return (not bool(bad.any())), float(err.max()), int(bad.sum())
+
+
+# ---- norms of q and k with rotation; caches held in 8 bits with a scale per block of tokens and head ----
+# Definitions in 64 bits, written from the formulas in include/minfer_attn.h.
+
+def norm_rope(x: torch.Tensor, weight, rotary_dim: int, base_freq: float, style: int, start, eps: float) -> torch.Tensor:
+    """x [B, L, H, D] -> float64: RMS norm of every head (weight [D], [H, D] or None for none), then the rotation by position start[b] + l."""
+    y = x.double()
+    if weight is not None:
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * weight.double()
+    half = rotary_dim // 2
+    pos = torch.as_tensor(start).double()[:, None] + torch.arange(x.size(1), dtype=torch.float64)
+    ang = pos[:, :, None, None] * base_freq ** (-2.0 * torch.arange(half, dtype=torch.float64) / max(rotary_dim, 1))
+    c, s = torch.cos(ang), torch.sin(ang)
+    out = y.clone()
+    lo, hi = (slice(0, rotary_dim, 2), slice(1, rotary_dim, 2)) if style == 0 else (slice(0, half), slice(half, rotary_dim))
+    out[..., lo] = y[..., lo] * c - y[..., hi] * s
+    out[..., hi] = y[..., lo] * s + y[..., hi] * c
+    return out
+
+
+def b8_scale(amax: torch.Tensor, int8: bool) -> torch.Tensor:
+    """The scale (float64, a value of float32) that blocks with these largest magnitudes need."""
+    amax = amax.double().clamp_max(torch.finfo(torch.float32).max)
+    least = 2.0 ** -126
+    if int8:
+        s = (amax / 127).float().double().clamp_min(least)
+    else:
+        m, e = torch.frexp(amax)                       # amax = m 2^e, m in [0.5, 1): 448 = 0.875 * 2^9
+        s = torch.ldexp(torch.ones_like(amax), e - 9 + (m > 0.875).int()).clamp_min(least)
+    return torch.where(amax > 0, s, torch.zeros_like(s))
+
+
+def b8_codes(x: torch.Tensor, scale: torch.Tensor, int8: bool) -> torch.Tensor:
+    """Nearest codes (as float64 values) of x under `scale` (broadcast), ties to even, saturated; NaN: kept (e4m3), 0 (int8)."""
+    s = scale.double().expand_as(x)
+    y = torch.where(s > 0, x.double() / s.clamp_min(1e-300), torch.zeros((), dtype=torch.float64))
+    if int8:
+        return torch.nan_to_num(torch.round(y).clamp(-127, 127), nan=0.0)
+    y = y.clamp(-448, 448)
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)      # eight values per binade, subnormals below 2^-6
+    return (torch.round(y / step) * step).clamp(-448, 448)
+
+
+def b8_append(codes: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, start: int, block: int, int8: bool):
+    """One head of one sequence: rows x [n, D] (float64) appended at row `start` of codes [rows, D] / scale [blocks] (float64 values).
+    Returns both as they are afterwards."""
+    codes, scale = codes.clone(), scale.clone()
+    p, end = start, start + x.size(0)
+    while p < end:
+        j = p // block
+        lo, hi = j * block, min((j + 1) * block, end)
+        new = x[p - start:hi - start]
+        finite = torch.nan_to_num(new.abs(), nan=0.0, posinf=torch.finfo(torch.float32).max)
+        old = scale[j] if p > lo else torch.zeros((), dtype=torch.float64)
+        s = torch.maximum(old, b8_scale(finite.max(), int8))
+        if p > lo and s != old:
+            codes[lo:p] = b8_codes((codes[lo:p] * old).float().double(), s, int8)
+        codes[p:hi] = b8_codes(new, s, int8)
+        scale[j] = s
+        p = hi
+    return codes, scale
+
+
+def b8_dequantize(codes: torch.Tensor, scale: torch.Tensor, block: int) -> torch.Tensor:
+    """codes [..., rows, D], scale [..., blocks] -> float64 values."""
+    return codes.double() * scale.double().repeat_interleave(block, -1)[..., :codes.size(-2), None]
+
+
+def b8_decode(q, k, v, lens, dtype):
+    """q [B, H, 1, D], k / v [B, Hkv, Lmax, D] float64 (dequantised), lens [B] -> (out float64, tolerance of a result in `dtype`).
+
+    The tolerance, element by element: weights rounded to fp16 (half a step, 2^-11 relative, of sum w |v|), the output's own rounding
+    (eps / 2), and the fp32 arithmetic: a score's sum of D products is off by at most 2^-20 of the sum of their magnitudes, which
+    moves its weight by that relative amount; exp2's approximation, the sums over keys and the merges by 2^-18 together."""
+    B, H, _, D = q.shape
+    Hkv = k.size(1)
+    out, tol = torch.zeros(B, H, 1, D, dtype=torch.float64), torch.zeros(B, H, 1, D, dtype=torch.float64)
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), k.size(2))
+        if n == 0:
+            continue
+        qb, kb, vb = q[b, :, 0].double().view(Hkv, H // Hkv, D), k[b, :, :n], v[b, :, :n]
+        t = qb @ kb.transpose(1, 2) / D ** 0.5
+        moved = (qb.abs() @ kb.abs().transpose(1, 2) / D ** 0.5).amax(-1, keepdim=True) * 2.0 ** -20
+        w = torch.softmax(t, -1)
+        o, mass = w @ vb, w @ vb.abs()
+        out[b, :, 0] = o.reshape(H, D)
+        tol[b, :, 0] = (mass * (2.0 ** -11 + 2.0 ** -18 + 2 * moved) + o.abs() * torch.finfo(dtype).eps / 2 + 2.0 ** -25).reshape(H, D)
+    return out, tol
