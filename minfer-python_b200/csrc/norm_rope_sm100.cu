@@ -28,7 +28,10 @@ namespace minfer_attn {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxAngles = 1024;  // (token, pair) angles a block keeps in shared memory
+constexpr int kMaxAngles = 1024;  // (token, pair) angles a block of rows keeps in shared memory
+constexpr int kStages = 4;        // rows of a thread on their way through shared memory (no registers held while they fly)
+constexpr int kStageVecs = 2 * kThreads;  // 16-byte pieces of a stage: two chunks per thread
+constexpr size_t kRowsSmem = 2 * kMaxAngles * sizeof(float) + kStages * kStageVecs * 16;
 
 template <bool BF16>
 __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
@@ -113,46 +116,26 @@ __device__ __forceinline__ void load_weights(const void* w, int kind, int c0, in
   }
 }
 
-// y = x / rms(x) * weight over the TPR lanes of a row (called by whole warps)
+// 1 / rms of a row, over its TPR lanes (called by whole warps)
 template <int TPR>
-__device__ __forceinline__ void norm_row(float* x, const float* w, bool live, float inv_dim, float eps) {
-  float ss = 0.f;
-  if (live) {
+__device__ __forceinline__ float inverse_rms(const float* x, bool live, float inv_dim, float eps) {
+  float ss = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+  for (int i = 0; i < 16; i += 2) {
+    ss = fmaf(x[i], x[i], ss);
+    s2 = fmaf(x[i + 1], x[i + 1], s2);
   }
+  ss = live ? ss + s2 : 0.f;
 #pragma unroll
   for (int d = TPR / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
-  const float r = rsqrtf(fmaf(ss, inv_dim, eps));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] *= r * w[i];
+  return rsqrtf(fmaf(ss, inv_dim, eps));
 }
 
+// x[e0], x[e1] of pair p (p = 0 .. 7): two halves (p, 8 + p), interleaved (2 p, 2 p + 1); pairs 0-3 and 4-7 of the latter lie in chunks 0 and 1
 template <bool kNeox>
-__device__ __forceinline__ void rotate_row(float* x, const Chunks<kNeox>& ch, const float* cs, const float* sn) {
-  if constexpr (kNeox) {
-    if (ch.rot0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float u = x[i], v = x[8 + i];
-        x[i] = u * cs[i] - v * sn[i];
-        x[8 + i] = u * sn[i] + v * cs[i];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h ? ch.rot1 : ch.rot0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u = x[8 * h + 2 * i], v = x[8 * h + 2 * i + 1];
-          x[8 * h + 2 * i] = u * cs[4 * h + i] - v * sn[4 * h + i];
-          x[8 * h + 2 * i + 1] = u * sn[4 * h + i] + v * cs[4 * h + i];
-        }
-      }
-    }
-  }
-}
+__device__ __forceinline__ constexpr int pair_lo(int p) { return kNeox ? p : 2 * p; }
+template <bool kNeox>
+__device__ __forceinline__ constexpr int pair_hi(int p) { return kNeox ? 8 + p : 2 * p + 1; }
 
 // the lane's eight angles out of a token's rows of cosines and sines
 template <bool kNeox>
@@ -200,11 +183,15 @@ __device__ __forceinline__ bool locate(const NormRopeArgs& a, int b, int pos, bo
 // ---- rows one by one: q, and k / v in place or into a 16-bit cache; with an 8-bit cache (kFmt) k and v of a call of one token per
 // sequence, whose row alone decides about its block ----
 //
-// A block takes 2^log_tb tokens; each token's rows are dealt out over the row groups it gets (and over `slices` blocks).
+// A block takes 2^log_tb tokens; each token's rows are dealt out over the row groups it gets (and over `slices` blocks).  A thread keeps
+// its token's angles, multiplied into the weights, in registers for all its rows (32 values; formed anew where the next row has other
+// weights), and its next rows on their way through shared memory.
 template <int TPR, bool BF16, bool kNeox, int kFmt>
-__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, unsigned slice, unsigned slices, int n_k, int n_v,
-                                          float* s_cos, float* s_sin) {
+__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, unsigned slice, unsigned slices, int n_k, int n_v, float* smem) {
   constexpr int kGroups = kThreads / TPR;
+  float* s_cos = smem;
+  float* s_sin = smem + kMaxAngles;
+  uint4* s_rows = reinterpret_cast<uint4*>(smem + 2 * kMaxAngles);
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int log_gpt = (31 - __clz(kGroups)) - a.log_tb;  // row groups per token, log2
@@ -218,11 +205,12 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, un
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int n_q = a.q != nullptr ? a.n_heads : 0;
   const int n_rows = n_q + n_k + n_v;
-  const uint8_t* q_base = reinterpret_cast<const uint8_t*>(a.q) + 2 * (static_cast<int64_t>(b) * a.q_stride[0] + static_cast<int64_t>(l) * a.q_stride[1]);
+  uint8_t* q_base = reinterpret_cast<uint8_t*>(a.q) + 2 * (static_cast<int64_t>(b) * a.q_stride[0] + static_cast<int64_t>(l) * a.q_stride[1]);
   const int64_t kv_off = 2 * (static_cast<int64_t>(b) * a.kv_stride[0] + static_cast<int64_t>(l) * a.kv_stride[1]);
   const int step = static_cast<int>(slices) << log_gpt;
   const int first = (static_cast<int>(slice) << log_gpt) + (rg & ((1 << log_gpt) - 1));
-  auto row_at = [&](int r, int& kind, int& h) -> const uint8_t* {
+  // kind 0: q, 1: k, 2: v
+  auto row_at = [&](int r, int& kind, int& h) -> uint8_t* {
     if (r < n_q) {
       kind = 0;
       h = r;
@@ -230,24 +218,23 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, un
     }
     kind = r < n_q + n_k ? 1 : 2;
     h = r - n_q - (kind == 2 ? n_k : 0);
-    return reinterpret_cast<const uint8_t*>(kind == 1 ? a.k : a.v) + kv_off + 2 * static_cast<int64_t>(h) * a.kv_stride[2];
+    return const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(kind == 1 ? a.k : a.v)) + kv_off + 2 * static_cast<int64_t>(h) * a.kv_stride[2];
   };
   // (all row groups of a block make the same number of steps, so that warps stay whole)
   const int n_steps = n_rows > static_cast<int>(slice << log_gpt) ? (n_rows - static_cast<int>(slice << log_gpt) + step - 1) / step : 0;
-  uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
-  int kind = 0, h = 0;
-  const uint8_t* src = nullptr;
-  auto fetch = [&](int r) {
-    src = nullptr;
-    if (token_ok && r < n_rows) {
-      src = row_at(r, kind, h);
-      if (ch.live) {
-        raw0 = *reinterpret_cast<const uint4*>(src + 16 * ch.c0);
-        raw1 = *reinterpret_cast<const uint4*>(src + 16 * ch.c1);
-      }
+  auto issue = [&](int it) {
+    const int r = first + it * step;
+    if (token_ok && ch.live && r < n_rows) {
+      int kind, h;
+      const uint8_t* src = row_at(r, kind, h);
+      uint4* dst = s_rows + (it % kStages) * kStageVecs + tid;
+      cp_async_16(dst, src + 16 * ch.c0, true);
+      cp_async_16(dst + kThreads, src + 16 * ch.c1, true);
     }
+    cp_async_commit();
   };
-  fetch(first);  // on its way before the position is known
+#pragma unroll
+  for (int it = 0; it < kStages - 1; ++it) issue(it);  // on their way before the position is known
 
   const int pos = (a.start != nullptr ? a.start[b] : a.start_pos) + l;
   // the block's angles, dealt out over its threads
@@ -266,54 +253,96 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, un
   if (a.k_cache != nullptr && n_k + n_v > 0 && token_ok && first + (n_steps - 1) * step >= n_q)  // (a thread with query rows alone needs no place)
     cache_ok = locate(a, b, pos, t == 0, outer, crow);
   __syncthreads();
-  float cs[8], sn[8];
-  load_angles<kNeox>(s_cos + tb * pairs, s_sin + tb * pairs, ch, cs, sn);
 
-  float w[16];
+  // y_lo = lo * m[0] - hi * m[1], y_hi = lo * m[2] + hi * m[3]
+  float m[4][8];
   const uint8_t* w_now = nullptr;
+  bool have = false;
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
   for (int it = 0; it < n_steps; ++it) {
-    const int kd = kind, hh = h;
-    const uint8_t* sp = src;
+    cp_async_wait<kStages - 2>();
+    const int r = first + it * step;
+    const bool row_ok = token_ok && r < n_rows;
+    int kind = 2, h = 0;
+    uint8_t* src = nullptr;
+    if (row_ok) src = row_at(r, kind, h);
+    uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
+    if (row_ok && ch.live) {
+      raw0 = s_rows[(it % kStages) * kStageVecs + tid];
+      raw1 = s_rows[(it % kStages) * kStageVecs + tid + kThreads];
+    }
+    issue(it + kStages - 1);
     float x[16];
     unpack8<BF16>(raw0, x);
     unpack8<BF16>(raw1, x + 8);
-    const uint4 v0 = raw0, v1 = raw1;
-    if (it + 1 < n_steps) fetch(first + (it + 1) * step);
-    if (a.q_weight != nullptr) {
-      if (sp != nullptr && kd != 2) {
-        const uint8_t* wp = kd == 0 ? reinterpret_cast<const uint8_t*>(a.q_weight) + static_cast<int64_t>(hh) * a.w_stride[0] * w_bytes
-                                    : reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(hh) * a.w_stride[1] * w_bytes;
-        if (wp != w_now) load_weights(wp, a.w_kind, ch.c0, ch.c1, w);
+    if (kind != 2) {
+      const uint8_t* wp = nullptr;
+      if (a.q_weight != nullptr)
+        wp = kind == 0 ? reinterpret_cast<const uint8_t*>(a.q_weight) + static_cast<int64_t>(h) * a.w_stride[0] * w_bytes
+                       : reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(h) * a.w_stride[1] * w_bytes;
+      if (!have || wp != w_now) {
+        float w[16], cs[8], sn[8];
+        if (wp != nullptr) {
+          load_weights(wp, a.w_kind, ch.c0, ch.c1, w);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = 1.f;
+        }
+        load_angles<kNeox>(s_cos + tb * pairs, s_sin + tb * pairs, ch, cs, sn);
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const bool rot = (kNeox || p < 4) ? ch.rot0 : ch.rot1;
+          const float c = rot ? cs[p] : 1.f, sv = rot ? sn[p] : 0.f;
+          m[0][p] = w[pair_lo<kNeox>(p)] * c;
+          m[1][p] = w[pair_hi<kNeox>(p)] * sv;
+          m[2][p] = w[pair_lo<kNeox>(p)] * sv;
+          m[3][p] = w[pair_hi<kNeox>(p)] * c;
+        }
         w_now = wp;
-      }
-      // (rows of v and idle groups take part in the shuffles of their warp)
-      float y[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = x[i];
-      norm_row<TPR>(y, w, ch.live, a.inv_dim, a.eps);
-      if (kd != 2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = y[i];
+        have = true;
       }
     }
-    if (kd != 2) rotate_row<kNeox>(x, ch, cs, sn);
+    if (a.q_weight != nullptr && __any_sync(0xFFFFFFFFu, kind != 2)) {
+      const float scale = inverse_rms<TPR>(x, ch.live, a.inv_dim, a.eps);
+      if (kind != 2) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= scale;
+      }
+    }
+    if (kind != 2) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        constexpr bool two_chunks = !kNeox;
+        const float lo = x[pair_lo<kNeox>(p)], hi = x[pair_hi<kNeox>(p)];
+        if ((two_chunks && p >= 4) ? ch.rot1 : ch.rot0) {
+          x[pair_lo<kNeox>(p)] = fmaf(lo, m[0][p], -(hi * m[1][p]));
+          x[pair_hi<kNeox>(p)] = fmaf(lo, m[2][p], hi * m[3][p]);
+        } else {  // (not 0 * hi: an infinite value stays in its place)
+          x[pair_lo<kNeox>(p)] = lo * m[0][p];
+          x[pair_hi<kNeox>(p)] = hi * m[3][p];
+        }
+      }
+    }
     if constexpr (kFmt == 0) {
-      if (sp == nullptr || !ch.live) continue;
-      uint8_t* dst = const_cast<uint8_t*>(sp);
-      if (kd != 0 && a.k_cache != nullptr) {
+      if (!row_ok || !ch.live) continue;
+      uint8_t* dst = src;
+      if (kind != 0 && a.k_cache != nullptr) {
         if (!cache_ok) continue;
-        dst = reinterpret_cast<uint8_t*>(kd == 1 ? a.k_cache : a.v_cache) +
-              2 * (static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(hh) * a.cache_stride[1] + static_cast<int64_t>(crow) * a.cache_stride[2]);
+        dst = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) +
+              2 * (static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow) * a.cache_stride[2]);
       }
-      *reinterpret_cast<uint4*>(dst + 16 * ch.c0) = kd == 2 ? v0 : pack8<BF16>(x);
-      *reinterpret_cast<uint4*>(dst + 16 * ch.c1) = kd == 2 ? v1 : pack8<BF16>(x + 8);
+      if (kind != 2) {
+        raw0 = pack8<BF16>(x);
+        raw1 = pack8<BF16>(x + 8);
+      }
+      *reinterpret_cast<uint4*>(dst + 16 * ch.c0) = raw0;
+      *reinterpret_cast<uint4*>(dst + 16 * ch.c1) = raw1;
     } else {
-      if (sp != nullptr && kd == 0 && ch.live) {
-        *reinterpret_cast<uint4*>(const_cast<uint8_t*>(sp) + 16 * ch.c0) = pack8<BF16>(x);
-        *reinterpret_cast<uint4*>(const_cast<uint8_t*>(sp) + 16 * ch.c1) = pack8<BF16>(x + 8);
+      if (row_ok && kind == 0 && ch.live) {
+        *reinterpret_cast<uint4*>(src + 16 * ch.c0) = pack8<BF16>(x);
+        *reinterpret_cast<uint4*>(src + 16 * ch.c1) = pack8<BF16>(x + 8);
       }
-      const bool cached = sp != nullptr && kd != 0 && cache_ok;
+      const bool cached = row_ok && kind != 0 && cache_ok;
       if (!__any_sync(0xFFFFFFFFu, cached)) continue;
       float amax = 0.f;
 #pragma unroll
@@ -324,9 +353,9 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, un
       uint8_t* blk_rows = nullptr;
       float s0 = 0.f, s1 = 0.f;
       if (cached) {
-        float* sc = (kd == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(hh) * a.scale_stride[1] + (crow >> a.log_block);
-        blk_rows = reinterpret_cast<uint8_t*>(kd == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
-                   static_cast<int64_t>(hh) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
+        float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
+        blk_rows = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
+                   static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
         s0 = begun != 0 ? *sc : 0.f;
         const float need = b8_scale<kFmt>(amax);
         s1 = s0 >= need ? s0 : need;
@@ -351,34 +380,39 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, un
 }
 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
-__global__ void __launch_bounds__(kThreads, TPR == 16 ? 2 : 3) norm_rope_rows_kernel(const NormRopeArgs a) {
-  __shared__ __align__(16) float s_cos[kMaxAngles];
-  __shared__ __align__(16) float s_sin[kMaxAngles];
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_rows_kernel(const NormRopeArgs a) {
+  __shared__ __align__(16) float s_all[kRowsSmem / 4];
   grid_launch_dependents();
   grid_dependency_wait();
-  rows_role<TPR, BF16, kNeox, kFmt>(a, blockIdx.x, blockIdx.y, gridDim.y, a.k != nullptr ? a.n_kv_heads : 0,
-                                    a.v != nullptr ? a.n_kv_heads : 0, s_cos, s_sin);
+  rows_role<TPR, BF16, kNeox, kFmt>(a, blockIdx.x, blockIdx.y, gridDim.y, a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_all);
 }
 
 // ---- blocks of an 8-bit cache: k and v of calls with several tokens per sequence ----
 //
-// A unit is one block of tokens of one sequence, for a slice of the kv heads, of k or of v: its rows are loaded, normed and rotated
-// into registers (fp32), the block's largest magnitude is agreed on, and the codes leave.  A head's rows of one block fill 2^log_block * TPR
-// lanes: four, two or one head at a time (kRows = 1), or two or four rows per thread.  The angles of a unit's tokens lie in
-// shared memory and serve all its heads.
-template <int TPR, bool BF16, bool kNeox, int kFmt, int kRows>
-__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, bool is_k, unsigned slice, unsigned slices, float* s_cos, float* s_sin,
-                                           float* s_max) {
+// A unit is one block of tokens of one sequence, for a slice of the kv heads, of k or of v.  A head's rows of one block fill 2^log_block * TPR
+// lanes: four, two or one head at a time, or two or four rows per thread.  The raw rows wait in shared memory (each thread's own
+// pieces: no barrier, and a piece is fetched for the next head as soon as its last reading is done), the angles of the unit's
+// tokens as well; the rows are normed and rotated twice, once for the block's largest magnitude and once for the codes, which
+// costs less than the registers or the shared memory that fp32 rows would take.
+template <int TPR, bool BF16, bool kNeox, int kFmt>
+__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, bool is_k, unsigned slice, unsigned slices, float* smem, float* s_max) {
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int blk = 1 << a.log_block;
+  const int pairs = a.rotary_dim / 2;
+  float* s_cos = smem;
+  float* s_sin = smem + (pairs << a.log_block);
+  float* s_norm = smem + (2 * pairs << a.log_block);             // 1 / rms of the rows of the heads at hand
+  const int rows = max(1, (blk * TPR) / kThreads);               // per thread
+  const int side = max(1, kThreads / (blk * TPR));               // heads side by side
+  uint4* s_raw = reinterpret_cast<uint4*>(s_norm + blk * side);  // [rows][2][kThreads]
   const int b = static_cast<int>(unit / static_cast<unsigned>(a.n_touch)), j = static_cast<int>(unit - static_cast<unsigned>(b) * static_cast<unsigned>(a.n_touch));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int64_t start = a.start != nullptr ? a.start[b] : a.start_pos;
   // the j-th block of those that the valid positions of this call touch
   const int64_t p0 = start > 0 ? start : 0, p1 = min(start + a.seq, static_cast<int64_t>(a.max_len));  // positions [p0, p1)
   if (tid == 0 && j == 0 && slice == 0 && is_k && (start < 0 || start + a.seq > a.max_len))
-    report(a.status, kStatusBadPosition, b, static_cast<int>(start < 0 ? start : start + a.seq - 1 > 0x7FFFFFFF ? 0x7FFFFFFF : max(start, static_cast<int64_t>(a.max_len))), a.max_len);
+    report(a.status, kStatusBadPosition, b, static_cast<int>(start < 0 ? start : max(start, static_cast<int64_t>(a.max_len))), a.max_len);
   const int64_t base64 = (p0 >> a.log_block << a.log_block) + static_cast<int64_t>(j) * blk;
   if (base64 >= p1) return;
   const int base = static_cast<int>(base64);
@@ -387,36 +421,25 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   if (!locate(a, b, base + lo, tid == 0 && is_k && slice == 0, outer, row0)) return;  // (a block lies in one page)
   row0 -= lo;
 
-  const int per_row_heads = kRows > 1 ? 1 : kThreads / (blk * TPR);  // heads side by side
-  const int sub = kRows > 1 ? 0 : rg >> a.log_block;                 // which of them
-  const int row_a = kRows > 1 ? rg * kRows : rg & (blk - 1);         // this lane's first row of the block
-  // heads of the slice
-  const int n_groups = (a.n_kv_heads + per_row_heads - 1) / per_row_heads;
+  const int sub = rg >> a.log_block;                                 // which of the heads side by side
+  const int row_a = rg & (blk - 1);                                  // this lane's rows of the block: row_a, row_a + row_step, ...
+  const int row_step = kThreads / TPR;
+  const int n_groups = (a.n_kv_heads + side - 1) / side;
   const int g0 = static_cast<int>(static_cast<unsigned>(n_groups) * slice / slices), g1 = static_cast<int>(static_cast<unsigned>(n_groups) * (slice + 1) / slices);
   const uint8_t* src_base = reinterpret_cast<const uint8_t*>(is_k ? a.k : a.v) + 2 * (static_cast<int64_t>(b) * a.kv_stride[0] + (base + row_a - start) * a.kv_stride[1]);
   uint8_t* cache = reinterpret_cast<uint8_t*>(is_k ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(row0) * a.cache_stride[2];
   float* scales = (is_k ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + (row0 >> a.log_block);
 
-  uint4 raw[kRows][2];
-  float s_old = 0.f;
-  auto fetch = [&](int g) {
-    const int h = g * per_row_heads + sub;
-    if (h < a.n_kv_heads) {
-      const uint8_t* p = src_base + 2 * static_cast<int64_t>(h) * a.kv_stride[2];
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        raw[r][0] = raw[r][1] = make_uint4(0, 0, 0, 0);
-        if (ch.live && row_a + r >= lo && row_a + r < hi) {
-          const uint8_t* q = p + 2 * static_cast<int64_t>(r) * a.kv_stride[1];
-          raw[r][0] = *reinterpret_cast<const uint4*>(q + 16 * ch.c0);
-          raw[r][1] = *reinterpret_cast<const uint4*>(q + 16 * ch.c1);
-        }
-      }
-      s_old = lo != 0 ? scales[static_cast<int64_t>(h) * a.scale_stride[1]] : 0.f;
+  auto fetch = [&](int g, int r) {
+    const int h = g * side + sub, row = row_a + r * row_step;
+    if (g < g1 && h < a.n_kv_heads && ch.live && row >= lo && row < hi) {
+      const uint8_t* p = src_base + 2 * (static_cast<int64_t>(h) * a.kv_stride[2] + static_cast<int64_t>(r) * row_step * a.kv_stride[1]);
+      cp_async_16(s_raw + (2 * r) * kThreads + tid, p + 16 * ch.c0, true);
+      cp_async_16(s_raw + (2 * r + 1) * kThreads + tid, p + 16 * ch.c1, true);
     }
   };
-  if (g0 < g1) fetch(g0);
-  const int pairs = a.rotary_dim / 2;
+  for (int r = 0; r < rows; ++r) fetch(g0, r);
+  cp_async_commit();
   if (is_k) {
     for (int u = tid + lo * pairs; u < hi * pairs; u += kThreads) {
       const int ut = u / pairs, i = u - ut * pairs;
@@ -426,64 +449,89 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     }
     __syncthreads();
   }
+  const bool norm = is_k && a.k_weight != nullptr;
   float w[16];
   const uint8_t* w_now = nullptr;
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
-  for (int g = g0; g < g1; ++g) {
-    const int h = g * per_row_heads + sub;
-    const bool head_ok = h < a.n_kv_heads;
-    float x[kRows][16];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      unpack8<BF16>(raw[r][0], x[r]);
-      unpack8<BF16>(raw[r][1], x[r] + 8);
+  // a row's values as they are to be coded; the first time with the row's 1 / rms found and kept
+  auto row_values = [&](int r, bool again, float (&x)[16]) {
+    const int row = row_a + r * row_step;
+    const bool mine = row >= lo && row < hi;
+    uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
+    if (mine && ch.live) {
+      raw0 = s_raw[(2 * r) * kThreads + tid];
+      raw1 = s_raw[(2 * r + 1) * kThreads + tid];
     }
-    const float s0 = s_old;
-    if (g + 1 < g1) fetch(g + 1);
-    float amax = 0.f;
-    if (is_k && a.k_weight != nullptr) {
+    unpack8<BF16>(raw0, x);
+    unpack8<BF16>(raw1, x + 8);
+    if (!is_k) return;
+    if (norm) {
+      float* kept = s_norm + sub * blk + row;
+      float f;
+      if (again) {
+        f = *kept;
+      } else {
+        f = inverse_rms<TPR>(x, ch.live, a.inv_dim, a.eps);
+        if (t == 0) *kept = f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= f * w[i];
+    }
+    if (mine) {
+      float cs[8], sn[8];
+      load_angles<kNeox>(s_cos + row * pairs, s_sin + row * pairs, ch, cs, sn);
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        if ((!kNeox && p >= 4) ? ch.rot1 : ch.rot0) {
+          const float u = x[pair_lo<kNeox>(p)], v = x[pair_hi<kNeox>(p)];
+          x[pair_lo<kNeox>(p)] = fmaf(u, cs[p], -(v * sn[p]));
+          x[pair_hi<kNeox>(p)] = fmaf(u, sn[p], v * cs[p]);
+        }
+      }
+    }
+  };
+  for (int g = g0; g < g1; ++g) {
+    const int h = g * side + sub;
+    const bool head_ok = h < a.n_kv_heads;
+    if (norm) {
       const uint8_t* wp = reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(head_ok ? h : 0) * a.w_stride[1] * w_bytes;
       if (wp != w_now) load_weights(wp, a.w_kind, ch.c0, ch.c1, w);
       w_now = wp;
     }
+    const float s0 = (head_ok && lo != 0) ? scales[static_cast<int64_t>(h) * a.scale_stride[1]] : 0.f;
+    cp_async_wait<0>();
+    float amax = 0.f;
+    for (int r = 0; r < rows; ++r) {
+      float x[16];
+      row_values(r, false, x);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      if (is_k) {
-        if (a.k_weight != nullptr) norm_row<TPR>(x[r], w, ch.live, a.inv_dim, a.eps);
-        if (row_a + r >= lo && row_a + r < hi) {
-          float cs[8], sn[8];
-          load_angles<kNeox>(s_cos + (row_a + r) * pairs, s_sin + (row_a + r) * pairs, ch, cs, sn);
-          rotate_row<kNeox>(x[r], ch, cs, sn);
-        }
-      }
-      if (row_a + r >= lo && row_a + r < hi) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[r][i]));
-      }
+      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));  // (rows that are not new: zeros)
     }
     // over the lanes that hold this head's rows: a warp's lanes, then the group's warps
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-    const int group_warps = kRows > 1 ? kThreads / 32 : (blk * TPR) / 32;
-    float* mine = s_max + (g & 1) * (kThreads / 32);  // two sets: one barrier per head
-    if ((tid & 31) == 0) mine[tid >> 5] = amax;
+    float* part = s_max + (g & 1) * (kThreads / 32);  // two sets: one barrier per head
+    if ((tid & 31) == 0) part[tid >> 5] = amax;
     __syncthreads();
     {
+      const int group_warps = min(kThreads, blk * TPR) / 32;
       const int w0 = (tid >> 5) / group_warps * group_warps;
-      for (int i = 0; i < group_warps; ++i) amax = fmaxf(amax, mine[w0 + i]);
+      for (int i = 0; i < group_warps; ++i) amax = fmaxf(amax, part[w0 + i]);
     }
-    if (!head_ok || !ch.live) continue;
     const float need = b8_scale<kFmt>(amax);
     const float s1 = s0 >= need ? s0 : need;
     const float r1 = b8_inverse(s1);
     uint8_t* dst = cache + static_cast<int64_t>(h) * a.cache_stride[1];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int row = row_a + r;
+    for (int r = 0; r < rows; ++r) {
+      const int row = row_a + r * row_step;
+      float x[16];
+      row_values(r, true, x);
+      fetch(g + 1, r);
+      if (!head_ok || !ch.live) continue;
       uint8_t* d = dst + static_cast<int64_t>(row) * a.cache_stride[2];
       if (row >= lo && row < hi) {
-        *reinterpret_cast<uint2*>(d + 8 * ch.c0) = b8_code8<kFmt>(x[r], s1, r1);
-        *reinterpret_cast<uint2*>(d + 8 * ch.c1) = b8_code8<kFmt>(x[r] + 8, s1, r1);
+        *reinterpret_cast<uint2*>(d + 8 * ch.c0) = b8_code8<kFmt>(x, s1, r1);
+        *reinterpret_cast<uint2*>(d + 8 * ch.c1) = b8_code8<kFmt>(x + 8, s1, r1);
       } else if (row < lo && s1 != s0) {  // rows that were there, under a scale that grew
         uint2* d0 = reinterpret_cast<uint2*>(d + 8 * ch.c0);
         uint2* d1 = reinterpret_cast<uint2*>(d + 8 * ch.c1);
@@ -492,29 +540,26 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
         *d1 = b8_recode8<kFmt>(y1, s0, s1, r1);
       }
     }
+    cp_async_commit();
     // one lane of the head's group
-    if (t == 0 && (kRows > 1 ? rg == 0 : (rg & (blk - 1)) == 0) && (lo == 0 || s1 != s0)) scales[static_cast<int64_t>(h) * a.scale_stride[1]] = s1;
+    if (head_ok && t == 0 && row_a == 0 && (lo == 0 || s1 != s0)) scales[static_cast<int64_t>(h) * a.scale_stride[1]] = s1;
   }
 }
 
 // Blocks [0, kv_blocks): units of k, then of v; behind them the query rows.
-template <int TPR, bool BF16, bool kNeox, int kFmt, int kRows>
+template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const NormRopeArgs a) {
-  extern __shared__ __align__(16) float s_angles[];
+  extern __shared__ __align__(16) float s_dyn[];
   __shared__ float s_max[2 * kThreads / 32];
   grid_launch_dependents();
   grid_dependency_wait();
-  const unsigned units = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch);
-  const unsigned kv_blocks = 2u * units * static_cast<unsigned>(a.slices);
-  if (blockIdx.x < kv_blocks) {
-    const unsigned per = units * static_cast<unsigned>(a.slices);
+  const unsigned per = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch) * static_cast<unsigned>(a.slices);  // blocks of k, and of v
+  if (blockIdx.x < 2 * per) {
     const bool is_k = blockIdx.x < per;
     const unsigned i = is_k ? blockIdx.x : blockIdx.x - per;
-    float* s_sin = s_angles + (a.rotary_dim / 2 << a.log_block);
-    block_role<TPR, BF16, kNeox, kFmt, kRows>(a, i / static_cast<unsigned>(a.slices), is_k, i % static_cast<unsigned>(a.slices), static_cast<unsigned>(a.slices),
-                                              s_angles, s_sin, s_max);
+    block_role<TPR, BF16, kNeox, kFmt>(a, i / static_cast<unsigned>(a.slices), is_k, i % static_cast<unsigned>(a.slices), static_cast<unsigned>(a.slices), s_dyn, s_max);
   } else {
-    rows_role<TPR, BF16, kNeox, 0>(a, blockIdx.x - kv_blocks, 0, 1, 0, 0, s_angles, s_angles + kMaxAngles);
+    rows_role<TPR, BF16, kNeox, 0>(a, blockIdx.x - 2 * per, 0, 1, 0, 0, s_dyn);
   }
 }
 
@@ -549,9 +594,9 @@ cudaError_t launch_rows(const NormRopeArgs& a, unsigned blocks, unsigned slices,
   return cudaLaunchKernelEx(&at.cfg, norm_rope_rows_kernel<TPR, BF16, kNeox, kFmt>, a);
 }
 
-template <int TPR, bool BF16, bool kNeox, int kFmt, int kRows>
+template <int TPR, bool BF16, bool kNeox, int kFmt>
 cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
-  auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt, kRows>;
+  auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt>;
   if (smem > 48 * 1024) {
     // (idempotent, and some hundred nanoseconds beside a call of many tokens)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -562,15 +607,6 @@ cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, c
   at.cfg.blockDim = dim3(kThreads);
   at.cfg.dynamicSmemBytes = smem;
   return cudaLaunchKernelEx(&at.cfg, kernel, a);
-}
-
-template <int TPR, bool BF16, bool kNeox, int kFmt>
-cudaError_t launch_blocks_rows(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
-  const int lanes = TPR << a.log_block;
-  if (lanes <= kThreads) return launch_blocks<TPR, BF16, kNeox, kFmt, 1>(a, blocks, smem, stream);
-  if (lanes == 2 * kThreads) return launch_blocks<TPR, BF16, kNeox, kFmt, 2>(a, blocks, smem, stream);
-  if constexpr (TPR == 8) return launch_blocks<TPR, BF16, kNeox, kFmt, 4>(a, blocks, smem, stream);
-  return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -623,11 +659,13 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   a.slices = static_cast<int>(slices);
   const long long blocks = 2 * units * slices + (a.q != nullptr ? blocks_x : 0);
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  size_t smem = static_cast<size_t>(a.rotary_dim / 2) * blk * 8;
-  if (smem < 2 * kMaxAngles * sizeof(float)) smem = 2 * kMaxAngles * sizeof(float);
+  // angles, 1 / rms, raw rows
+  size_t smem = static_cast<size_t>(a.rotary_dim / 2) * blk * 8 + static_cast<size_t>(blk) * side * 4 +
+                static_cast<size_t>((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads) * 32;
+  if (a.q != nullptr && smem < kRowsSmem) smem = kRowsSmem;
   const unsigned nb = static_cast<unsigned>(blocks);
-  if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks_rows, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks_rows, 8, kE4M3, a, nb, smem, stream);
-  return tpr == 4 ? MINFER_NR_STYLE(launch_blocks_rows, 4, kInt8, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks_rows, 8, kInt8, a, nb, smem, stream);
+  if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kE4M3, a, nb, smem, stream);
+  return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kInt8, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kInt8, a, nb, smem, stream);
 #undef MINFER_NR_STYLE
 }
 
