@@ -162,9 +162,9 @@ struct NormRopeArgs {
   float eps;
   // set by the launcher
   float inv_dim;
-  int32_t log_tb;           // tokens per block of rows, log2
+  int32_t slices;           // warps per token
   int32_t n_touch;          // blocks of tokens that a sequence's new rows can touch
-  int32_t slices;           // thread blocks per (sequence, block of tokens) of k, and of v
+  int32_t kv_slices;        // thread blocks per (sequence, block of tokens) of k, and of v
   uint64_t turns[128];      // frequencies: turns per position, as fractions of 2^64
 };
 // cache_format: MINFER_ATTN_KV_16BIT, _E4M3 or _INT8

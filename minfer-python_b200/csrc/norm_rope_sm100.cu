@@ -20,6 +20,7 @@
 #include "ptx.cuh"
 
 #include <cmath>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -27,11 +28,11 @@ namespace minfer_attn {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxAngles = 1024;  // (token, pair) angles a block of rows keeps in shared memory
-constexpr int kStages = 4;        // rows of a thread on their way through shared memory (no registers held while they fly)
-constexpr int kStageVecs = 2 * kThreads;  // 16-byte pieces of a stage: two chunks per thread
-constexpr size_t kRowsSmem = 2 * kMaxAngles * sizeof(float) + kStages * kStageVecs * 16;
+constexpr int kRowThreads = 128;    // a block that works on rows
+constexpr int kThreads = 256;       // a block that works on blocks of a cache (and, behind those, on rows)
+constexpr int kMaxPairs = 128;      // rotated pairs of a head
+constexpr int kStages = 3;  // steps of two rows per thread on their way through shared memory (no registers held while they fly)
+constexpr int rows_smem(int threads) { return kStages * 4 * threads * static_cast<int>(sizeof(uint4)); }
 
 template <bool BF16>
 __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
@@ -116,37 +117,133 @@ __device__ __forceinline__ void load_weights(const void* w, int kind, int c0, in
   }
 }
 
-// 1 / rms of a row, over its TPR lanes (called by whole warps)
-template <int TPR>
-__device__ __forceinline__ float inverse_rms(const float* x, bool live, float inv_dim, float eps) {
-  float ss = 0.f, s2 = 0.f;
+// A lane's 16 values of a row as eight pairs (lo, hi): two halves (x[p], x[8 + p]), interleaved (x[2 p], x[2 p + 1]) with pairs 0-3 in
+// chunk c0 and 4-7 in chunk c1; two pairs to a register pair, so that the arithmetic goes two values at a time.
+struct Pairs {
+  float2 lo[4], hi[4];
+};
+
+template <bool kNeox>
+__device__ __forceinline__ Pairs as_pairs(const float* x) {
+  Pairs r;
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    ss = fmaf(x[i], x[i], ss);
-    s2 = fmaf(x[i + 1], x[i + 1], s2);
+  for (int i = 0; i < 4; ++i) {
+    r.lo[i] = kNeox ? make_float2(x[2 * i], x[2 * i + 1]) : make_float2(x[4 * i], x[4 * i + 2]);
+    r.hi[i] = kNeox ? make_float2(x[8 + 2 * i], x[9 + 2 * i]) : make_float2(x[4 * i + 1], x[4 * i + 3]);
   }
-  ss = live ? ss + s2 : 0.f;
+  return r;
+}
+template <bool kNeox>
+__device__ __forceinline__ void as_values(const Pairs& r, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[kNeox ? 2 * i : 4 * i] = r.lo[i].x;
+    x[kNeox ? 2 * i + 1 : 4 * i + 2] = r.lo[i].y;
+    x[kNeox ? 8 + 2 * i : 4 * i + 1] = r.hi[i].x;
+    x[kNeox ? 9 + 2 * i : 4 * i + 3] = r.hi[i].y;
+  }
+}
+
+// 1 / rms of a row, over its TPR lanes (called by whole warps; lanes without a chunk hold zeros)
+template <int TPR>
+__device__ __forceinline__ float inverse_rms(const Pairs& x, float inv_dim, float eps) {
+  float2 s = __fmul2_rn(x.lo[0], x.lo[0]), u = __fmul2_rn(x.hi[0], x.hi[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    s = __ffma2_rn(x.lo[i], x.lo[i], s);
+    u = __ffma2_rn(x.hi[i], x.hi[i], u);
+  }
+  s = __fadd2_rn(s, u);
+  float ss = s.x + s.y;
 #pragma unroll
   for (int d = TPR / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
   return rsqrtf(fmaf(ss, inv_dim, eps));
 }
 
-// x[e0], x[e1] of pair p (p = 0 .. 7): two halves (p, 8 + p), interleaved (2 p, 2 p + 1); pairs 0-3 and 4-7 of the latter lie in chunks 0 and 1
+__device__ __forceinline__ void scale_pairs(Pairs& x, float f) {
+  const float2 f2 = make_float2(f, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.lo[i] = __fmul2_rn(x.lo[i], f2);
+    x.hi[i] = __fmul2_rn(x.hi[i], f2);
+  }
+}
+
+// A lane's angles; pairs that are not rotated are left out by apply_angles, not turned by 0 (an infinite value stays in its place).
+struct Angles {
+  float2 c[4], s[4], n[4];  // cos, sin, -sin
+};
+
 template <bool kNeox>
-__device__ __forceinline__ constexpr int pair_lo(int p) { return kNeox ? p : 2 * p; }
+__device__ __forceinline__ void apply_angles(Pairs& x, const Angles& g, const Chunks<kNeox>& ch) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((!kNeox && i >= 2) ? ch.rot1 : ch.rot0) {
+      const float2 lo = x.lo[i], hi = x.hi[i];
+      x.lo[i] = __ffma2_rn(hi, g.n[i], __fmul2_rn(lo, g.c[i]));
+      x.hi[i] = __ffma2_rn(lo, g.s[i], __fmul2_rn(hi, g.c[i]));
+    }
+  }
+}
+
 template <bool kNeox>
-__device__ __forceinline__ constexpr int pair_hi(int p) { return kNeox ? 8 + p : 2 * p + 1; }
+__device__ __forceinline__ Pairs weight_pairs(const void* w, int w_kind, const Chunks<kNeox>& ch) {
+  float f[16];
+  load_weights(w, w_kind, ch.c0, ch.c1, f);
+  return as_pairs<kNeox>(f);
+}
+
+// x * f * weight
+__device__ __forceinline__ void apply_weights(Pairs& x, const Pairs& w, float f) {
+  scale_pairs(x, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x.lo[i] = __fmul2_rn(x.lo[i], w.lo[i]);
+    x.hi[i] = __fmul2_rn(x.hi[i], w.hi[i]);
+  }
+}
 
 // the lane's eight angles out of a token's rows of cosines and sines
 template <bool kNeox>
-__device__ __forceinline__ void load_angles(const float* cosines, const float* sines, const Chunks<kNeox>& ch, float* cs, float* sn) {
-  if (ch.rot0) {
-    *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(cosines + ch.i0);
-    *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(sines + ch.i0);
+__device__ __forceinline__ void load_angles(const float* cosines, const float* sines, const Chunks<kNeox>& ch, Angles& g) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h ? ch.rot1 : ch.rot0) {
+      const float4 c = *reinterpret_cast<const float4*>(cosines + (h ? ch.i1 : ch.i0)), s = *reinterpret_cast<const float4*>(sines + (h ? ch.i1 : ch.i0));
+      g.c[2 * h] = make_float2(c.x, c.y);
+      g.c[2 * h + 1] = make_float2(c.z, c.w);
+      g.s[2 * h] = make_float2(s.x, s.y);
+      g.s[2 * h + 1] = make_float2(s.z, s.w);
+      g.n[2 * h] = make_float2(-s.x, -s.y);
+      g.n[2 * h + 1] = make_float2(-s.z, -s.w);
+    }
   }
-  if (ch.rot1) {
-    *reinterpret_cast<float4*>(cs + 4) = *reinterpret_cast<const float4*>(cosines + ch.i1);
-    *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(sines + ch.i1);
+}
+
+// The same computed by a warp whose row groups all work for one token: each group takes its share of a lane's eight angles.
+template <int TPR, bool kNeox>
+__device__ __forceinline__ void warp_angles(const NormRopeArgs& a, int pos, const Chunks<kNeox>& ch, int t, int group, Angles& g) {
+  constexpr int kShare = 8 / (32 / TPR);  // angles per group: 1, 2 or 4
+  float2 mine[kShare];
+#pragma unroll
+  for (int u = 0; u < kShare; ++u) {
+    const int p = group * kShare + u;
+    const int i = p < 4 ? ch.i0 + p : ch.i1 + p - 4;
+    mine[u] = angle_of(a, pos, min(i, kMaxPairs - 1));  // (lanes and pairs beyond rotary_dim: some angle that nobody uses)
+  }
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const int from = (p / kShare) * TPR + t;
+    const float c = __shfl_sync(0xFFFFFFFFu, mine[p % kShare].x, from), s = __shfl_sync(0xFFFFFFFFu, mine[p % kShare].y, from);
+    if (p & 1) {
+      g.c[p / 2].y = c;
+      g.s[p / 2].y = s;
+      g.n[p / 2].y = -s;
+    } else {
+      g.c[p / 2].x = c;
+      g.s[p / 2].x = s;
+      g.n[p / 2].x = -s;
+    }
   }
 }
 
@@ -183,226 +280,230 @@ __device__ __forceinline__ bool locate(const NormRopeArgs& a, int b, int pos, bo
 // ---- rows one by one: q, and k / v in place or into a 16-bit cache; with an 8-bit cache (kFmt) k and v of a call of one token per
 // sequence, whose row alone decides about its block ----
 //
-// A block takes 2^log_tb tokens; each token's rows are dealt out over the row groups it gets (and over `slices` blocks).  A thread keeps
-// its token's angles, multiplied into the weights, in registers for all its rows (32 values; formed anew where the next row has other
-// weights), and its next rows on their way through shared memory.
-template <int TPR, bool BF16, bool kNeox, int kFmt>
-__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned bx, unsigned slice, unsigned slices, int n_k, int n_v, float* smem) {
-  constexpr int kGroups = kThreads / TPR;
-  float* s_cos = smem;
-  float* s_sin = smem + kMaxAngles;
-  uint4* s_rows = reinterpret_cast<uint4*>(smem + 2 * kMaxAngles);
+// A warp takes a token (or, with few tokens, one of `slices` shares of its rows): nothing is shared between warps, no barrier.  Its
+// 32 / TPR row groups walk the query heads, the k heads and the v heads side by side, two rows each per step (two independent chains
+// of reduction and arithmetic).  A thread brings its own pieces of the next steps into shared memory with asynchronous copies.  The
+// token's angles stay in registers for all rows, the weights too unless every head has its own.
+struct Cursor {  // of one row group: its two rows of a step
+  int s, row, n;
+  int kind;            // 0 q, 1 k, 2 v
+  int64_t off, step;   // bytes from the kind's base: of the first row, between its two rows
+};
+
+template <int TPR, bool BF16, bool kNeox, int kFmt, int kT>
+__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, unsigned slices, int n_k, int n_v, uint4* s_rows) {
+  constexpr int kSide = 32 / TPR;  // row groups of a warp
   const int tid = static_cast<int>(threadIdx.x);
-  const int t = tid % TPR, rg = tid / TPR;
-  const int log_gpt = (31 - __clz(kGroups)) - a.log_tb;  // row groups per token, log2
-  const unsigned n_tokens = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.seq);
-  const unsigned token0 = bx << a.log_tb;
-  const int tb = rg >> log_gpt;
-  const bool token_ok = token0 + tb < n_tokens;
-  const unsigned token = token_ok ? token0 + tb : n_tokens - 1;
+  const int lane = tid & 31;
+  const int t = lane % TPR, group = lane / TPR;
+  const unsigned token = item / slices, slice = item - token * slices;
+  if (token >= static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.seq)) return;
   const int b = static_cast<int>(token / static_cast<unsigned>(a.seq));
   const int l = static_cast<int>(token - static_cast<unsigned>(b) * static_cast<unsigned>(a.seq));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int n_q = a.q != nullptr ? a.n_heads : 0;
-  const int n_rows = n_q + n_k + n_v;
+  // steps of 2 kSide rows: q's, k's, v's; this warp's are [s0, s1)
+  const int q_steps = (n_q + 2 * kSide - 1) / (2 * kSide), k_steps = (n_k + 2 * kSide - 1) / (2 * kSide), v_steps = (n_v + 2 * kSide - 1) / (2 * kSide);
+  const int steps = q_steps + k_steps + v_steps;
+  const int s0 = static_cast<int>(static_cast<unsigned>(steps) * slice / slices), s1 = static_cast<int>(static_cast<unsigned>(steps) * (slice + 1) / slices);
   uint8_t* q_base = reinterpret_cast<uint8_t*>(a.q) + 2 * (static_cast<int64_t>(b) * a.q_stride[0] + static_cast<int64_t>(l) * a.q_stride[1]);
   const int64_t kv_off = 2 * (static_cast<int64_t>(b) * a.kv_stride[0] + static_cast<int64_t>(l) * a.kv_stride[1]);
-  const int step = static_cast<int>(slices) << log_gpt;
-  const int first = (static_cast<int>(slice) << log_gpt) + (rg & ((1 << log_gpt) - 1));
-  // kind 0: q, 1: k, 2: v
-  auto row_at = [&](int r, int& kind, int& h) -> uint8_t* {
-    if (r < n_q) {
-      kind = 0;
-      h = r;
-      return q_base + 2 * static_cast<int64_t>(h) * a.q_stride[2];
-    }
-    kind = r < n_q + n_k ? 1 : 2;
-    h = r - n_q - (kind == 2 ? n_k : 0);
-    return const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(kind == 1 ? a.k : a.v)) + kv_off + 2 * static_cast<int64_t>(h) * a.kv_stride[2];
+  uint8_t* k_base = const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(a.k)) + kv_off;
+  const uint8_t* v_base = reinterpret_cast<const uint8_t*>(a.v) + kv_off;
+
+  auto enter = [&](Cursor& c) {  // the kind that step c.s belongs to
+    c.kind = c.s < q_steps ? 0 : c.s < q_steps + k_steps ? 1 : 2;
+    c.row = (c.s - (c.kind == 0 ? 0 : c.kind == 1 ? q_steps : q_steps + k_steps)) * 2 * kSide + group;
+    c.n = c.kind == 0 ? n_q : c.kind == 1 ? n_k : n_v;
+    const int64_t stride = 2 * (c.kind == 0 ? a.q_stride[2] : a.kv_stride[2]);
+    c.off = c.row * stride;
+    c.step = stride * kSide;
   };
-  // (all row groups of a block make the same number of steps, so that warps stay whole)
-  const int n_steps = n_rows > static_cast<int>(slice << log_gpt) ? (n_rows - static_cast<int>(slice << log_gpt) + step - 1) / step : 0;
-  auto issue = [&](int it) {
-    const int r = first + it * step;
-    if (token_ok && ch.live && r < n_rows) {
-      int kind, h;
-      const uint8_t* src = row_at(r, kind, h);
-      uint4* dst = s_rows + (it % kStages) * kStageVecs + tid;
-      cp_async_16(dst, src + 16 * ch.c0, true);
-      cp_async_16(dst + kThreads, src + 16 * ch.c1, true);
+  auto advance = [&](Cursor& c) {
+    ++c.s;
+    c.row += 2 * kSide;
+    c.off += 2 * c.step;
+    if (c.s == q_steps || c.s == q_steps + k_steps) enter(c);
+  };
+  Cursor in;  // the step to be fetched next
+  in.s = s0;
+  enter(in);
+  auto issue = [&](int stage) {
+    if (in.s < s1) {
+      const uint8_t* src = (in.kind == 0 ? q_base : in.kind == 1 ? k_base : v_base) + in.off;
+      uint4* dst = s_rows + stage * 4 * kT + tid;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (ch.live && in.row + u * kSide < in.n) {
+          cp_async_16(dst + (2 * u) * kT, src + u * in.step + 16 * ch.c0, true);
+          cp_async_16(dst + (2 * u + 1) * kT, src + u * in.step + 16 * ch.c1, true);
+        }
+      }
+      advance(in);
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int it = 0; it < kStages - 1; ++it) issue(it);  // on their way before the position is known
+  for (int i = 0; i < kStages - 1; ++i) issue(i);  // on their way before the position is known
 
   const int pos = (a.start != nullptr ? a.start[b] : a.start_pos) + l;
-  // the block's angles, dealt out over its threads
-  const int pairs = a.rotary_dim / 2;
-  for (int u = tid; u < (pairs << a.log_tb); u += kThreads) {
-    const int ut = u / pairs, i = u - ut * pairs;
-    const unsigned utok = min(token0 + ut, n_tokens - 1);
-    const int ub = static_cast<int>(utok / static_cast<unsigned>(a.seq));
-    const int up = (a.start != nullptr ? a.start[ub] : a.start_pos) + static_cast<int>(utok - static_cast<unsigned>(ub) * static_cast<unsigned>(a.seq));
-    const float2 cs = angle_of(a, up, i);
-    s_cos[u] = cs.x;
-    s_sin[u] = cs.y;
-  }
   int outer = 0, crow = 0;
   bool cache_ok = false;
-  if (a.k_cache != nullptr && n_k + n_v > 0 && token_ok && first + (n_steps - 1) * step >= n_q)  // (a thread with query rows alone needs no place)
-    cache_ok = locate(a, b, pos, t == 0, outer, crow);
-  __syncthreads();
-
-  // y_lo = lo * m[0] - hi * m[1], y_hi = lo * m[2] + hi * m[3]
-  float m[4][8];
-  const uint8_t* w_now = nullptr;
-  bool have = false;
+  if (a.k_cache != nullptr && s1 > q_steps) cache_ok = locate(a, b, pos, lane == 0, outer, crow);
+  Angles angles = {};
+  if (s0 < q_steps + k_steps && a.rotary_dim > 0) warp_angles<TPR, kNeox>(a, pos, ch, t, group, angles);
+  Pairs weights = {};
+  int weights_of = -1;  // kind
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
-  for (int it = 0; it < n_steps; ++it) {
+
+  Cursor at;
+  at.s = s0;
+  enter(at);
+  int stage = 0;
+  for (; at.s < s1; advance(at)) {
     cp_async_wait<kStages - 2>();
-    const int r = first + it * step;
-    const bool row_ok = token_ok && r < n_rows;
-    int kind = 2, h = 0;
-    uint8_t* src = nullptr;
-    if (row_ok) src = row_at(r, kind, h);
-    uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
-    if (row_ok && ch.live) {
-      raw0 = s_rows[(it % kStages) * kStageVecs + tid];
-      raw1 = s_rows[(it % kStages) * kStageVecs + tid + kThreads];
+    const uint4* sp = s_rows + stage * 4 * kT + tid;
+    const bool both = at.row - group + kSide < at.n;  // rows for the second half of the step
+    uint4 raw[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool there = ch.live && at.row + u * kSide < at.n;
+      raw[u][0] = there ? sp[(2 * u) * kT] : make_uint4(0, 0, 0, 0);
+      raw[u][1] = there ? sp[(2 * u + 1) * kT] : make_uint4(0, 0, 0, 0);
     }
-    issue(it + kStages - 1);
-    float x[16];
-    unpack8<BF16>(raw0, x);
-    unpack8<BF16>(raw1, x + 8);
+    issue(stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+    const int kind = at.kind;
+    float x[2][16];
+    auto turn = [&](auto rows) {  // norm, weights and rotation of one row or two
+      constexpr int kRows = decltype(rows)::value;
+      const int64_t w_stride = (kind == 0 ? a.w_stride[0] : a.w_stride[1]) * w_bytes;
+      const uint8_t* w = reinterpret_cast<const uint8_t*>(kind == 0 ? a.q_weight : a.k_weight);
+      Pairs y[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        unpack8<BF16>(raw[u][0], x[u]);
+        unpack8<BF16>(raw[u][1], x[u] + 8);
+        y[u] = as_pairs<kNeox>(x[u]);
+      }
+      if (w != nullptr) {
+        if (w_stride == 0 && weights_of != kind) {
+          weights = weight_pairs<kNeox>(w, a.w_kind, ch);
+          weights_of = kind;
+        }
+        float f[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) f[u] = inverse_rms<TPR>(y[u], a.inv_dim, a.eps);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+          if (w_stride != 0) weights = weight_pairs<kNeox>(w + min(at.row + u * kSide, at.n - 1) * w_stride, a.w_kind, ch);
+          apply_weights(y[u], weights, f[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        apply_angles<kNeox>(y[u], angles, ch);
+        as_values<kNeox>(y[u], x[u]);
+        if (kFmt == 0 || kind == 0) {
+          raw[u][0] = pack8<BF16>(x[u]);
+          raw[u][1] = pack8<BF16>(x[u] + 8);
+        }
+      }
+    };
     if (kind != 2) {
-      const uint8_t* wp = nullptr;
-      if (a.q_weight != nullptr)
-        wp = kind == 0 ? reinterpret_cast<const uint8_t*>(a.q_weight) + static_cast<int64_t>(h) * a.w_stride[0] * w_bytes
-                       : reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(h) * a.w_stride[1] * w_bytes;
-      if (!have || wp != w_now) {
-        float w[16], cs[8], sn[8];
-        if (wp != nullptr) {
-          load_weights(wp, a.w_kind, ch.c0, ch.c1, w);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 1.f;
-        }
-        load_angles<kNeox>(s_cos + tb * pairs, s_sin + tb * pairs, ch, cs, sn);
-#pragma unroll
-        for (int p = 0; p < 8; ++p) {
-          const bool rot = (kNeox || p < 4) ? ch.rot0 : ch.rot1;
-          const float c = rot ? cs[p] : 1.f, sv = rot ? sn[p] : 0.f;
-          m[0][p] = w[pair_lo<kNeox>(p)] * c;
-          m[1][p] = w[pair_hi<kNeox>(p)] * sv;
-          m[2][p] = w[pair_lo<kNeox>(p)] * sv;
-          m[3][p] = w[pair_hi<kNeox>(p)] * c;
-        }
-        w_now = wp;
-        have = true;
-      }
+      if (both) turn(std::integral_constant<int, 2>{});
+      else turn(std::integral_constant<int, 1>{});
     }
-    if (a.q_weight != nullptr && __any_sync(0xFFFFFFFFu, kind != 2)) {
-      const float scale = inverse_rms<TPR>(x, ch.live, a.inv_dim, a.eps);
-      if (kind != 2) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= scale;
-      }
-    }
-    if (kind != 2) {
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        constexpr bool two_chunks = !kNeox;
-        const float lo = x[pair_lo<kNeox>(p)], hi = x[pair_hi<kNeox>(p)];
-        if ((two_chunks && p >= 4) ? ch.rot1 : ch.rot0) {
-          x[pair_lo<kNeox>(p)] = fmaf(lo, m[0][p], -(hi * m[1][p]));
-          x[pair_hi<kNeox>(p)] = fmaf(lo, m[2][p], hi * m[3][p]);
-        } else {  // (not 0 * hi: an infinite value stays in its place)
-          x[pair_lo<kNeox>(p)] = lo * m[0][p];
-          x[pair_hi<kNeox>(p)] = hi * m[3][p];
-        }
-      }
-    }
-    if constexpr (kFmt == 0) {
-      if (!row_ok || !ch.live) continue;
-      uint8_t* dst = src;
-      if (kind != 0 && a.k_cache != nullptr) {
+    if (kFmt == 0 || kind == 0) {
+      uint8_t* dst;
+      int64_t dst_step;
+      if (kind == 0 || a.k_cache == nullptr) {
+        dst = (kind == 0 ? q_base : k_base) + at.off;
+        dst_step = at.step;
+      } else {
         if (!cache_ok) continue;
         dst = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) +
-              2 * (static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow) * a.cache_stride[2]);
+              2 * (static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(at.row) * a.cache_stride[1] + static_cast<int64_t>(crow) * a.cache_stride[2]);
+        dst_step = 2 * kSide * a.cache_stride[1];
       }
-      if (kind != 2) {
-        raw0 = pack8<BF16>(x);
-        raw1 = pack8<BF16>(x + 8);
-      }
-      *reinterpret_cast<uint4*>(dst + 16 * ch.c0) = raw0;
-      *reinterpret_cast<uint4*>(dst + 16 * ch.c1) = raw1;
-    } else {
-      if (row_ok && kind == 0 && ch.live) {
-        *reinterpret_cast<uint4*>(src + 16 * ch.c0) = pack8<BF16>(x);
-        *reinterpret_cast<uint4*>(src + 16 * ch.c1) = pack8<BF16>(x + 8);
-      }
-      const bool cached = row_ok && kind != 0 && cache_ok;
-      if (!__any_sync(0xFFFFFFFFu, cached)) continue;
-      float amax = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
-#pragma unroll
-      for (int d = TPR / 2; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+      for (int u = 0; u < 2; ++u) {
+        if (!ch.live || at.row + u * kSide >= at.n) continue;
+        *reinterpret_cast<uint4*>(dst + u * dst_step + 16 * ch.c0) = raw[u][0];
+        *reinterpret_cast<uint4*>(dst + u * dst_step + 16 * ch.c1) = raw[u][1];
+      }
+    } else if constexpr (kFmt != 0) {
+      if (!cache_ok) continue;
       const int begun = crow & ((1 << a.log_block) - 1);  // rows of the block that are there
-      uint8_t* blk_rows = nullptr;
-      float s0 = 0.f, s1 = 0.f;
-      if (cached) {
-        float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
-        blk_rows = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
-                   static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
-        s0 = begun != 0 ? *sc : 0.f;
-        const float need = b8_scale<kFmt>(amax);
-        s1 = s0 >= need ? s0 : need;
-        const float r1 = b8_inverse(s1);
-        uint8_t* dst = blk_rows + static_cast<int64_t>(begun) * a.cache_stride[2];
-        *reinterpret_cast<uint2*>(dst + 8 * ch.c0) = b8_code8<kFmt>(x, s1, r1);
-        *reinterpret_cast<uint2*>(dst + 8 * ch.c1) = b8_code8<kFmt>(x + 8, s1, r1);
-        if (t == 0 && (begun == 0 || s1 != s0)) *sc = s1;  // (a block that begins here held anything)
-      }
-      // A scale that grew: the rows before are coded again, by the whole warp
-      unsigned grown = __ballot_sync(0xFFFFFFFFu, cached && begun != 0 && s1 != s0 && t == 0);
-      while (grown != 0) {
-        const int from = __ffs(grown) - 1;
-        grown &= grown - 1;
-        const uint64_t p = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(blk_rows), from);
-        const float o0 = __shfl_sync(0xFFFFFFFFu, s0, from), o1 = __shfl_sync(0xFFFFFFFFu, s1, from);
-        const int n = __shfl_sync(0xFFFFFFFFu, begun, from);
-        recode_rows<kFmt>(reinterpret_cast<uint8_t*>(p), a.cache_stride[2], n, a.head_dim / 16, o0, o1, tid & 31, 32);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u == 1 && !both) break;
+        if (kind == 2) {
+          unpack8<BF16>(raw[u][0], x[u]);
+          unpack8<BF16>(raw[u][1], x[u] + 8);
+        }
+        const int h = at.row + u * kSide;
+        const bool row_ok = h < at.n;
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[u][i]));
+#pragma unroll
+        for (int d = TPR / 2; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
+        uint8_t* blk_rows = nullptr;
+        float o0 = 0.f, o1 = 0.f;                           // the block's scale before and after
+        if (row_ok) {
+          float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
+          blk_rows = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
+                     static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
+          o0 = begun != 0 ? *sc : 0.f;
+          const float need = b8_scale<kFmt>(amax);
+          o1 = o0 >= need ? o0 : need;
+          const float r1 = b8_inverse(o1);
+          uint8_t* dst = blk_rows + static_cast<int64_t>(begun) * a.cache_stride[2];
+          *reinterpret_cast<uint2*>(dst + 8 * ch.c0) = b8_code8<kFmt>(x[u], o1, r1);
+          *reinterpret_cast<uint2*>(dst + 8 * ch.c1) = b8_code8<kFmt>(x[u] + 8, o1, r1);
+          if (t == 0 && (begun == 0 || o1 != o0)) *sc = o1;  // (a block that begins here held anything)
+        }
+        // A scale that grew: the rows before are coded again, by the whole warp
+        unsigned grown = __ballot_sync(0xFFFFFFFFu, row_ok && begun != 0 && o1 != o0 && t == 0);
+        while (grown != 0) {
+          const int from = __ffs(grown) - 1;
+          grown &= grown - 1;
+          const uint64_t p = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(blk_rows), from);
+          recode_rows<kFmt>(reinterpret_cast<uint8_t*>(p), a.cache_stride[2], begun, a.head_dim / 16, __shfl_sync(0xFFFFFFFFu, o0, from),
+                            __shfl_sync(0xFFFFFFFFu, o1, from), lane, 32);
+        }
       }
     }
   }
 }
 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
-__global__ void __launch_bounds__(kThreads, 2) norm_rope_rows_kernel(const NormRopeArgs a) {
-  __shared__ __align__(16) float s_all[kRowsSmem / 4];
+__global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const NormRopeArgs a) {
+  __shared__ __align__(16) uint4 s_rows[rows_smem(kRowThreads) / sizeof(uint4)];
   grid_launch_dependents();
   grid_dependency_wait();
-  rows_role<TPR, BF16, kNeox, kFmt>(a, blockIdx.x, blockIdx.y, gridDim.y, a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_all);
+  rows_role<TPR, BF16, kNeox, kFmt, kRowThreads>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
+                                                 a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_rows);
 }
 
 // ---- blocks of an 8-bit cache: k and v of calls with several tokens per sequence ----
 //
 // A unit is one block of tokens of one sequence, for a slice of the kv heads, of k or of v.  A head's rows of one block fill 2^log_block * TPR
 // lanes: four, two or one head at a time, or two or four rows per thread.  The raw rows wait in shared memory (each thread's own
-// pieces: no barrier, and a piece is fetched for the next head as soon as its last reading is done), the angles of the unit's
-// tokens as well; the rows are normed and rotated twice, once for the block's largest magnitude and once for the codes, which
-// costs less than the registers or the shared memory that fp32 rows would take.
+// pieces: no barrier, and a piece is fetched for the next head as soon as its last reading is done); the rows are normed and
+// rotated twice, once for the block's largest magnitude and once for the codes, which costs less than the registers or the shared
+// memory that fp32 rows would take.  A thread computes the angles of its first row once for all heads of the unit and turns them on
+// from row to row by the angle between two of its rows (three times at most, an error of 2^-24 each).
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, bool is_k, unsigned slice, unsigned slices, float* smem, float* s_max) {
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int blk = 1 << a.log_block;
   const int pairs = a.rotary_dim / 2;
-  float* s_cos = smem;
-  float* s_sin = smem + (pairs << a.log_block);
-  float* s_norm = smem + (2 * pairs << a.log_block);             // 1 / rms of the rows of the heads at hand
+  float* s_cos = smem;                                           // of the angle between two rows of a thread
+  float* s_sin = smem + kMaxPairs;
+  float* s_norm = smem + 2 * kMaxPairs;                          // 1 / rms of the rows of the heads at hand
   const int rows = max(1, (blk * TPR) / kThreads);               // per thread
   const int side = max(1, kThreads / (blk * TPR));               // heads side by side
   uint4* s_raw = reinterpret_cast<uint4*>(s_norm + blk * side);  // [rows][2][kThreads]
@@ -440,21 +541,43 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   };
   for (int r = 0; r < rows; ++r) fetch(g0, r);
   cp_async_commit();
-  if (is_k) {
-    for (int u = tid + lo * pairs; u < hi * pairs; u += kThreads) {
-      const int ut = u / pairs, i = u - ut * pairs;
-      const float2 cs = angle_of(a, base + ut, i);
-      s_cos[u] = cs.x;
-      s_sin[u] = cs.y;
+  Angles first = {};
+  if (is_k && pairs > 0) {
+    if (rows > 1) {
+      for (int u = tid; u < pairs; u += kThreads) {
+        const float2 cs = angle_of(a, row_step, u);
+        s_cos[u] = cs.x;
+        s_sin[u] = cs.y;
+      }
+      __syncthreads();
     }
-    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (p < 4 ? ch.rot0 : ch.rot1) {
+        const float2 cs = angle_of(a, base + row_a, p < 4 ? ch.i0 + p : ch.i1 + p - 4);
+        (p & 1 ? first.c[p / 2].y : first.c[p / 2].x) = cs.x;
+        (p & 1 ? first.s[p / 2].y : first.s[p / 2].x) = cs.y;
+        (p & 1 ? first.n[p / 2].y : first.n[p / 2].x) = -cs.y;
+      }
+    }
   }
+  auto next_row = [&](Angles& g) {
+    Angles d = {};
+    load_angles<kNeox>(s_cos, s_sin, ch, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 c = g.c[i];
+      g.c[i] = __ffma2_rn(g.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
+      g.s[i] = __ffma2_rn(g.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
+      g.n[i] = make_float2(-g.s[i].x, -g.s[i].y);
+    }
+  };
   const bool norm = is_k && a.k_weight != nullptr;
-  float w[16];
+  Pairs weights = {};
   const uint8_t* w_now = nullptr;
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
   // a row's values as they are to be coded; the first time with the row's 1 / rms found and kept
-  auto row_values = [&](int r, bool again, float (&x)[16]) {
+  auto row_values = [&](int r, bool again, const Angles& angles, float (&x)[16]) {
     const int row = row_a + r * row_step;
     const bool mine = row >= lo && row < hi;
     uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
@@ -465,45 +588,37 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     unpack8<BF16>(raw0, x);
     unpack8<BF16>(raw1, x + 8);
     if (!is_k) return;
+    Pairs y = as_pairs<kNeox>(x);
     if (norm) {
       float* kept = s_norm + sub * blk + row;
       float f;
       if (again) {
         f = *kept;
       } else {
-        f = inverse_rms<TPR>(x, ch.live, a.inv_dim, a.eps);
+        f = inverse_rms<TPR>(y, a.inv_dim, a.eps);
         if (t == 0) *kept = f;
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= f * w[i];
+      apply_weights(y, weights, f);
     }
-    if (mine) {
-      float cs[8], sn[8];
-      load_angles<kNeox>(s_cos + row * pairs, s_sin + row * pairs, ch, cs, sn);
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        if ((!kNeox && p >= 4) ? ch.rot1 : ch.rot0) {
-          const float u = x[pair_lo<kNeox>(p)], v = x[pair_hi<kNeox>(p)];
-          x[pair_lo<kNeox>(p)] = fmaf(u, cs[p], -(v * sn[p]));
-          x[pair_hi<kNeox>(p)] = fmaf(u, sn[p], v * cs[p]);
-        }
-      }
-    }
+    apply_angles<kNeox>(y, angles, ch);
+    as_values<kNeox>(y, x);
   };
   for (int g = g0; g < g1; ++g) {
     const int h = g * side + sub;
     const bool head_ok = h < a.n_kv_heads;
     if (norm) {
       const uint8_t* wp = reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(head_ok ? h : 0) * a.w_stride[1] * w_bytes;
-      if (wp != w_now) load_weights(wp, a.w_kind, ch.c0, ch.c1, w);
+      if (wp != w_now) weights = weight_pairs<kNeox>(wp, a.w_kind, ch);
       w_now = wp;
     }
     const float s0 = (head_ok && lo != 0) ? scales[static_cast<int64_t>(h) * a.scale_stride[1]] : 0.f;
     cp_async_wait<0>();
     float amax = 0.f;
+    Angles angles = first;
     for (int r = 0; r < rows; ++r) {
       float x[16];
-      row_values(r, false, x);
+      if (is_k && r > 0) next_row(angles);
+      row_values(r, false, angles, x);
 #pragma unroll
       for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));  // (rows that are not new: zeros)
     }
@@ -522,10 +637,12 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     const float s1 = s0 >= need ? s0 : need;
     const float r1 = b8_inverse(s1);
     uint8_t* dst = cache + static_cast<int64_t>(h) * a.cache_stride[1];
+    angles = first;
     for (int r = 0; r < rows; ++r) {
       const int row = row_a + r * row_step;
       float x[16];
-      row_values(r, true, x);
+      if (is_k && r > 0) next_row(angles);
+      row_values(r, true, angles, x);
       fetch(g + 1, r);
       if (!head_ok || !ch.live) continue;
       uint8_t* d = dst + static_cast<int64_t>(row) * a.cache_stride[2];
@@ -546,20 +663,21 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   }
 }
 
-// Blocks [0, kv_blocks): units of k, then of v; behind them the query rows.
+// Blocks of threads: units of k, then of v; behind them the query rows.
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const NormRopeArgs a) {
   extern __shared__ __align__(16) float s_dyn[];
   __shared__ float s_max[2 * kThreads / 32];
   grid_launch_dependents();
   grid_dependency_wait();
-  const unsigned per = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch) * static_cast<unsigned>(a.slices);  // blocks of k, and of v
+  const unsigned per = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch) * static_cast<unsigned>(a.kv_slices);  // blocks of k, and of v
   if (blockIdx.x < 2 * per) {
     const bool is_k = blockIdx.x < per;
     const unsigned i = is_k ? blockIdx.x : blockIdx.x - per;
-    block_role<TPR, BF16, kNeox, kFmt>(a, i / static_cast<unsigned>(a.slices), is_k, i % static_cast<unsigned>(a.slices), static_cast<unsigned>(a.slices), s_dyn, s_max);
+    block_role<TPR, BF16, kNeox, kFmt>(a, i / static_cast<unsigned>(a.kv_slices), is_k, i % static_cast<unsigned>(a.kv_slices), static_cast<unsigned>(a.kv_slices), s_dyn, s_max);
   } else {
-    rows_role<TPR, BF16, kNeox, 0>(a, blockIdx.x - 2 * per, 0, 1, 0, 0, s_dyn);
+    rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - 2 * per) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
+                                             reinterpret_cast<uint4*>(s_dyn));
   }
 }
 
@@ -567,10 +685,10 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
 void fill_turns(NormRopeArgs& a, double freq_base) {
   thread_local double cached_base = 0.0;
   thread_local int cached_rot = -1;
-  thread_local uint64_t table[128];
+  thread_local uint64_t table[kMaxPairs];
   if (cached_base != freq_base || cached_rot != a.rotary_dim) {
     const long double two_pi = 6.283185307179586476925286766559005768L;
-    for (int i = 0; i < 128; ++i) {
+    for (int i = 0; i < kMaxPairs; ++i) {
       if (i >= a.rotary_dim / 2) {
         table[i] = 0;
         continue;
@@ -583,21 +701,21 @@ void fill_turns(NormRopeArgs& a, double freq_base) {
     cached_base = freq_base;
     cached_rot = a.rotary_dim;
   }
-  for (int i = 0; i < 128; ++i) a.turns[i] = table[i];
+  for (int i = 0; i < kMaxPairs; ++i) a.turns[i] = table[i];
 }
 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
-cudaError_t launch_rows(const NormRopeArgs& a, unsigned blocks, unsigned slices, cudaStream_t stream) {
+cudaError_t launch_rows(const NormRopeArgs& a, unsigned blocks, cudaStream_t stream) {
   LaunchAttrs at(stream);
-  at.cfg.gridDim = dim3(blocks, slices);
-  at.cfg.blockDim = dim3(kThreads);
+  at.cfg.gridDim = dim3(blocks);
+  at.cfg.blockDim = dim3(kRowThreads);
   return cudaLaunchKernelEx(&at.cfg, norm_rope_rows_kernel<TPR, BF16, kNeox, kFmt>, a);
 }
 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
   auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt>;
-  if (smem > 48 * 1024) {
+  if (smem > 47 * 1024) {  // (48 KB with the static part)
     // (idempotent, and some hundred nanoseconds beside a call of many tokens)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
@@ -616,53 +734,50 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   fill_turns(a, freq_base);
   a.inv_dim = 1.0f / static_cast<float>(a.head_dim);
   const int tpr = a.head_dim <= 64 ? 4 : a.head_dim <= 128 ? 8 : 16;
-  const int groups = kThreads / tpr;
+  const int side = 32 / tpr;  // row groups of a warp
   const long long tokens = static_cast<long long>(a.batch) * a.seq;
   const int fmt = cache_format == MINFER_ATTN_KV_E4M3 ? kE4M3 : cache_format == MINFER_ATTN_KV_INT8 ? kInt8 : 0;
   const bool by_block = fmt != 0 && a.seq > 1;
-  const int n_kv = by_block ? 0 : (a.k != nullptr ? a.n_kv_heads : 0) + (a.v != nullptr ? a.n_kv_heads : 0);
-  const int n_rows = (a.q != nullptr ? a.n_heads : 0) + n_kv;
-  // Tokens per block: more share the block's set-up, fewer fill the GPU.
-  a.log_tb = 0;
-  const int max_tb = a.rotary_dim > 0 ? kMaxAngles / (a.rotary_dim / 2) : groups;
-  while ((4 << a.log_tb) <= groups && (2 << a.log_tb) <= max_tb && (tokens >> (a.log_tb + 1)) >= 4 * 148) ++a.log_tb;
-  const long long blocks_x = (tokens + (1 << a.log_tb) - 1) >> a.log_tb;
+  const int kv_rows = by_block ? 0 : a.n_kv_heads;
+  const int step_rows = 2 * side;
+  const int steps = (a.q != nullptr ? (a.n_heads + step_rows - 1) / step_rows : 0) + (a.k != nullptr ? (kv_rows + step_rows - 1) / step_rows : 0) +
+                    (a.v != nullptr ? (kv_rows + step_rows - 1) / step_rows : 0);
+  // A warp takes a token; while that leaves the GPU's warps (16 per SM) without work, a token's rows are dealt out over several.
+  long long slices = (16 * 148 + tokens - 1) / tokens;
+  if (slices > steps) slices = steps;
+  if (slices < 1) slices = 1;
+  a.slices = static_cast<int>(slices);
+  const int row_warps = (by_block ? kThreads : kRowThreads) / 32;
+  const long long row_blocks = (tokens * slices + row_warps - 1) / row_warps;
 #define MINFER_NR_STYLE(fn, TPR, F, ...) \
   (bf16 ? (neox ? fn<TPR, true, true, F>(__VA_ARGS__) : fn<TPR, true, false, F>(__VA_ARGS__)) \
         : (neox ? fn<TPR, false, true, F>(__VA_ARGS__) : fn<TPR, false, false, F>(__VA_ARGS__)))
   if (!by_block) {
-    // few tokens: a token's rows over several blocks, one row per group
-    long long slices = 1;
-    if (a.log_tb == 0) {
-      slices = (n_rows + groups - 1) / groups;
-      if (slices * blocks_x > 8 * 148) slices = (8 * 148 + blocks_x - 1) / blocks_x;
-      if (slices < 1) slices = 1;
-    }
-    const unsigned bx = static_cast<unsigned>(blocks_x), sl = static_cast<unsigned>(slices);
+    const unsigned nb = static_cast<unsigned>(row_blocks);
     if (fmt == 0) {
-      if (tpr == 4) return MINFER_NR_STYLE(launch_rows, 4, 0, a, bx, sl, stream);
-      if (tpr == 8) return MINFER_NR_STYLE(launch_rows, 8, 0, a, bx, sl, stream);
-      return MINFER_NR_STYLE(launch_rows, 16, 0, a, bx, sl, stream);
+      if (tpr == 4) return MINFER_NR_STYLE(launch_rows, 4, 0, a, nb, stream);
+      if (tpr == 8) return MINFER_NR_STYLE(launch_rows, 8, 0, a, nb, stream);
+      return MINFER_NR_STYLE(launch_rows, 16, 0, a, nb, stream);
     }
-    if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_rows, 4, kE4M3, a, bx, sl, stream) : MINFER_NR_STYLE(launch_rows, 8, kE4M3, a, bx, sl, stream);
-    return tpr == 4 ? MINFER_NR_STYLE(launch_rows, 4, kInt8, a, bx, sl, stream) : MINFER_NR_STYLE(launch_rows, 8, kInt8, a, bx, sl, stream);
+    if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_rows, 4, kE4M3, a, nb, stream) : MINFER_NR_STYLE(launch_rows, 8, kE4M3, a, nb, stream);
+    return tpr == 4 ? MINFER_NR_STYLE(launch_rows, 4, kInt8, a, nb, stream) : MINFER_NR_STYLE(launch_rows, 8, kInt8, a, nb, stream);
   }
   const int blk = 1 << a.log_block;
   a.n_touch = (a.seq + blk - 2) / blk + 1;
   const long long units = static_cast<long long>(a.batch) * a.n_touch;
-  const int side = (tpr << a.log_block) < kThreads ? kThreads / (tpr << a.log_block) : 1;  // heads side by side
-  const int head_groups = (a.n_kv_heads + side - 1) / side;
+  const int abreast = (tpr << a.log_block) < kThreads ? kThreads / (tpr << a.log_block) : 1;  // heads side by side
+  const int head_groups = (a.n_kv_heads + abreast - 1) / abreast;
   // heads of a unit over several blocks while the GPU is not full
-  long long slices = (4 * 148 + units - 1) / units;
-  if (slices > head_groups) slices = head_groups;
-  if (slices < 1) slices = 1;
-  a.slices = static_cast<int>(slices);
-  const long long blocks = 2 * units * slices + (a.q != nullptr ? blocks_x : 0);
+  long long kv_slices = (4 * 148 + units - 1) / units;
+  if (kv_slices > head_groups) kv_slices = head_groups;
+  if (kv_slices < 1) kv_slices = 1;
+  a.kv_slices = static_cast<int>(kv_slices);
+  const long long blocks = 2 * units * kv_slices + (a.q != nullptr ? row_blocks : 0);
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  // angles, 1 / rms, raw rows
-  size_t smem = static_cast<size_t>(a.rotary_dim / 2) * blk * 8 + static_cast<size_t>(blk) * side * 4 +
+  // angles between rows, 1 / rms, raw rows
+  size_t smem = 2 * kMaxPairs * sizeof(float) + static_cast<size_t>(blk) * abreast * 4 +
                 static_cast<size_t>((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads) * 32;
-  if (a.q != nullptr && smem < kRowsSmem) smem = kRowsSmem;
+  if (a.q != nullptr && smem < static_cast<size_t>(rows_smem(kThreads))) smem = rows_smem(kThreads);
   const unsigned nb = static_cast<unsigned>(blocks);
   if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kE4M3, a, nb, smem, stream);
   return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kInt8, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kInt8, a, nb, smem, stream);
