@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t int8_to_half2(uint32_t src) {
   return *reinterpret_cast<const uint32_t*>(&q);
 }
 
-// eight values -> eight codes
+// eight values -> eight codes; r = 1 / s
 template <int kFmt>
 __device__ __forceinline__ uint2 b8_code8(const float* x, float s, float r) {
   uint32_t w[2];
@@ -83,7 +83,9 @@ __device__ __forceinline__ uint2 b8_code8(const float* x, float s, float r) {
   for (int i = 0; i < 2; ++i) {
     const float* y = x + 4 * i;
     if constexpr (kFmt == kE4M3) {
-      w[i] = e4m3_pair(y[0] * r, y[1] * r) | (e4m3_pair(y[2] * r, y[3] * r) << 16);
+      const float2 r2 = make_float2(r, r);
+      const float2 u = __fmul2_rn(make_float2(y[0], y[1]), r2), v = __fmul2_rn(make_float2(y[2], y[3]), r2);
+      w[i] = e4m3_pair(u.x, u.y) | (e4m3_pair(v.x, v.y) << 16);
     } else {
       w[i] = int8_code(y[0], s, r) | (int8_code(y[1], s, r) << 8) | (int8_code(y[2], s, r) << 16) | (int8_code(y[3], s, r) << 24);
     }

@@ -490,36 +490,56 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const No
 // ---- blocks of an 8-bit cache: k and v of calls with several tokens per sequence ----
 //
 // A unit is one block of tokens of one sequence, for a slice of the kv heads, of k or of v.  A head's rows of one block fill 2^log_block * TPR
-// lanes: four, two or one head at a time, or two or four rows per thread.  The raw rows wait in shared memory (each thread's own
-// pieces: no barrier, and a piece is fetched for the next head as soon as its last reading is done); the rows are normed and
-// rotated twice, once for the block's largest magnitude and once for the codes, which costs less than the registers or the shared
-// memory that fp32 rows would take.  A thread computes the angles of its first row once for all heads of the unit and turns them on
-// from row to row by the angle between two of its rows (three times at most, an error of 2^-24 each).
-template <int TPR, bool BF16, bool kNeox, int kFmt>
-__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, bool is_k, unsigned slice, unsigned slices, float* smem, float* s_max) {
+// lanes: four, two or one head at a time, or two or four rows per thread.  The raw rows come through shared memory, each thread's own
+// pieces (no barrier; the next head's are fetched as soon as these have been read); k's normed and rotated rows wait there in
+// fp32 until the block's largest magnitude is agreed on.  A thread computes the angles of its first row once for all heads of the
+// unit and turns them on from row to row by the angle between two of its rows (three times at most, an error of 2^-24 each).
+constexpr int blocks_smem(int lanes, bool k) {  // lanes that the rows of the heads side by side fill (kThreads at least)
+  return 2 * kMaxPairs * 4 + lanes * 32 + (k ? lanes * 64 : 0);
+}
+
+// largest magnitude of a row's raw values (NaN is passed over)
+template <bool BF16>
+__device__ __forceinline__ float raw_amax(const uint4& p, const uint4& q) {
+  const uint32_t w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+  if constexpr (BF16) {
+    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
+template <int TPR, bool BF16, bool kNeox, int kFmt, bool kIsK>
+__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, unsigned slice, unsigned slices, float* smem, float* s_max) {
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int blk = 1 << a.log_block;
   const int pairs = a.rotary_dim / 2;
-  float* s_cos = smem;                                           // of the angle between two rows of a thread
-  float* s_sin = smem + kMaxPairs;
-  float* s_norm = smem + 2 * kMaxPairs;                          // 1 / rms of the rows of the heads at hand
   const int rows = max(1, (blk * TPR) / kThreads);               // per thread
   const int side = max(1, kThreads / (blk * TPR));               // heads side by side
-  uint4* s_raw = reinterpret_cast<uint4*>(s_norm + blk * side);  // [rows][2][kThreads]
+  float* s_cos = smem;                                           // of the angle between two rows of a thread
+  float* s_sin = smem + kMaxPairs;
+  uint4* s_raw = reinterpret_cast<uint4*>(smem + 2 * kMaxPairs) + tid;                    // [rows][2] pieces, kThreads apart
+  float4* s_val = reinterpret_cast<float4*>(smem + 2 * kMaxPairs) + rows * 2 * kThreads + tid;  // [rows][4]: k as it is to be coded
   const int b = static_cast<int>(unit / static_cast<unsigned>(a.n_touch)), j = static_cast<int>(unit - static_cast<unsigned>(b) * static_cast<unsigned>(a.n_touch));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int64_t start = a.start != nullptr ? a.start[b] : a.start_pos;
   // the j-th block of those that the valid positions of this call touch
   const int64_t p0 = start > 0 ? start : 0, p1 = min(start + a.seq, static_cast<int64_t>(a.max_len));  // positions [p0, p1)
-  if (tid == 0 && j == 0 && slice == 0 && is_k && (start < 0 || start + a.seq > a.max_len))
+  if (kIsK && tid == 0 && j == 0 && slice == 0 && (start < 0 || start + a.seq > a.max_len))
     report(a.status, kStatusBadPosition, b, static_cast<int>(start < 0 ? start : max(start, static_cast<int64_t>(a.max_len))), a.max_len);
   const int64_t base64 = (p0 >> a.log_block << a.log_block) + static_cast<int64_t>(j) * blk;
   if (base64 >= p1) return;
   const int base = static_cast<int>(base64);
   const int lo = static_cast<int>(max(p0 - base, static_cast<int64_t>(0))), hi = static_cast<int>(min(p1 - base, static_cast<int64_t>(blk)));  // new rows of the block
   int outer, row0;
-  if (!locate(a, b, base + lo, tid == 0 && is_k && slice == 0, outer, row0)) return;  // (a block lies in one page)
+  if (!locate(a, b, base + lo, kIsK && tid == 0 && slice == 0, outer, row0)) return;  // (a block lies in one page)
   row0 -= lo;
 
   const int sub = rg >> a.log_block;                                 // which of the heads side by side
@@ -527,22 +547,24 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   const int row_step = kThreads / TPR;
   const int n_groups = (a.n_kv_heads + side - 1) / side;
   const int g0 = static_cast<int>(static_cast<unsigned>(n_groups) * slice / slices), g1 = static_cast<int>(static_cast<unsigned>(n_groups) * (slice + 1) / slices);
-  const uint8_t* src_base = reinterpret_cast<const uint8_t*>(is_k ? a.k : a.v) + 2 * (static_cast<int64_t>(b) * a.kv_stride[0] + (base + row_a - start) * a.kv_stride[1]);
-  uint8_t* cache = reinterpret_cast<uint8_t*>(is_k ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(row0) * a.cache_stride[2];
-  float* scales = (is_k ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + (row0 >> a.log_block);
+  const int64_t src_step = 2 * row_step * a.kv_stride[1], dst_step = row_step * a.cache_stride[2];
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(kIsK ? a.k : a.v) + 2 * (static_cast<int64_t>(b) * a.kv_stride[0] + (base + row_a - start) * a.kv_stride[1]);
+  uint8_t* cache = reinterpret_cast<uint8_t*>(kIsK ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] + static_cast<int64_t>(row0 + row_a) * a.cache_stride[2];
+  float* scales = (kIsK ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + (row0 >> a.log_block);
 
+  auto is_new = [&](int r) { return row_a + r * row_step >= lo && row_a + r * row_step < hi; };
   auto fetch = [&](int g, int r) {
-    const int h = g * side + sub, row = row_a + r * row_step;
-    if (g < g1 && h < a.n_kv_heads && ch.live && row >= lo && row < hi) {
-      const uint8_t* p = src_base + 2 * (static_cast<int64_t>(h) * a.kv_stride[2] + static_cast<int64_t>(r) * row_step * a.kv_stride[1]);
-      cp_async_16(s_raw + (2 * r) * kThreads + tid, p + 16 * ch.c0, true);
-      cp_async_16(s_raw + (2 * r + 1) * kThreads + tid, p + 16 * ch.c1, true);
+    const int h = g * side + sub;
+    if (g < g1 && h < a.n_kv_heads && ch.live && is_new(r)) {
+      const uint8_t* p = src + 2 * static_cast<int64_t>(h) * a.kv_stride[2] + r * src_step;
+      cp_async_16(s_raw + (2 * r) * kThreads, p + 16 * ch.c0, true);
+      cp_async_16(s_raw + (2 * r + 1) * kThreads, p + 16 * ch.c1, true);
     }
   };
   for (int r = 0; r < rows; ++r) fetch(g0, r);
   cp_async_commit();
   Angles first = {};
-  if (is_k && pairs > 0) {
+  if (kIsK && pairs > 0) {
     if (rows > 1) {
       for (int u = tid; u < pairs; u += kThreads) {
         const float2 cs = angle_of(a, row_step, u);
@@ -561,52 +583,13 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
       }
     }
   }
-  auto next_row = [&](Angles& g) {
-    Angles d = {};
-    load_angles<kNeox>(s_cos, s_sin, ch, d);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 c = g.c[i];
-      g.c[i] = __ffma2_rn(g.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
-      g.s[i] = __ffma2_rn(g.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
-      g.n[i] = make_float2(-g.s[i].x, -g.s[i].y);
-    }
-  };
-  const bool norm = is_k && a.k_weight != nullptr;
   Pairs weights = {};
   const uint8_t* w_now = nullptr;
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
-  // a row's values as they are to be coded; the first time with the row's 1 / rms found and kept
-  auto row_values = [&](int r, bool again, const Angles& angles, float (&x)[16]) {
-    const int row = row_a + r * row_step;
-    const bool mine = row >= lo && row < hi;
-    uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;
-    if (mine && ch.live) {
-      raw0 = s_raw[(2 * r) * kThreads + tid];
-      raw1 = s_raw[(2 * r + 1) * kThreads + tid];
-    }
-    unpack8<BF16>(raw0, x);
-    unpack8<BF16>(raw1, x + 8);
-    if (!is_k) return;
-    Pairs y = as_pairs<kNeox>(x);
-    if (norm) {
-      float* kept = s_norm + sub * blk + row;
-      float f;
-      if (again) {
-        f = *kept;
-      } else {
-        f = inverse_rms<TPR>(y, a.inv_dim, a.eps);
-        if (t == 0) *kept = f;
-      }
-      apply_weights(y, weights, f);
-    }
-    apply_angles<kNeox>(y, angles, ch);
-    as_values<kNeox>(y, x);
-  };
   for (int g = g0; g < g1; ++g) {
     const int h = g * side + sub;
     const bool head_ok = h < a.n_kv_heads;
-    if (norm) {
+    if (kIsK && a.k_weight != nullptr) {
       const uint8_t* wp = reinterpret_cast<const uint8_t*>(a.k_weight) + static_cast<int64_t>(head_ok ? h : 0) * a.w_stride[1] * w_bytes;
       if (wp != w_now) weights = weight_pairs<kNeox>(wp, a.w_kind, ch);
       w_now = wp;
@@ -616,12 +599,43 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     float amax = 0.f;
     Angles angles = first;
     for (int r = 0; r < rows; ++r) {
-      float x[16];
-      if (is_k && r > 0) next_row(angles);
-      row_values(r, false, angles, x);
+      uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;  // (rows that are not new: zeros)
+      if (is_new(r) && ch.live) {
+        raw0 = s_raw[(2 * r) * kThreads];
+        raw1 = s_raw[(2 * r + 1) * kThreads];
+      }
+      if constexpr (!kIsK) {
+        amax = fmaxf(amax, raw_amax<BF16>(raw0, raw1));
+      } else {
+        fetch(g + 1, r);
+        if (r > 0) {  // the angles of the thread's next row
+          Angles d = {};
+          load_angles<kNeox>(s_cos, s_sin, ch, d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));  // (rows that are not new: zeros)
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = angles.c[i];
+            angles.c[i] = __ffma2_rn(angles.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
+            angles.s[i] = __ffma2_rn(angles.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
+            angles.n[i] = make_float2(-angles.s[i].x, -angles.s[i].y);
+          }
+        }
+        float x[16];
+        unpack8<BF16>(raw0, x);
+        unpack8<BF16>(raw1, x + 8);
+        Pairs y = as_pairs<kNeox>(x);
+        if (a.k_weight != nullptr) apply_weights(y, weights, inverse_rms<TPR>(y, a.inv_dim, a.eps));
+        apply_angles<kNeox>(y, angles, ch);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          amax = fmax3(amax, fabsf(y.lo[i].x), fabsf(y.lo[i].y));
+          amax = fmax3(amax, fabsf(y.hi[i].x), fabsf(y.hi[i].y));
+        }
+        as_values<kNeox>(y, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_val[(4 * r + i) * kThreads] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      }
     }
+    if (kIsK) cp_async_commit();
     // over the lanes that hold this head's rows: a warp's lanes, then the group's warps
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
@@ -637,33 +651,34 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     const float s1 = s0 >= need ? s0 : need;
     const float r1 = b8_inverse(s1);
     uint8_t* dst = cache + static_cast<int64_t>(h) * a.cache_stride[1];
-    angles = first;
     for (int r = 0; r < rows; ++r) {
-      const int row = row_a + r * row_step;
-      float x[16];
-      if (is_k && r > 0) next_row(angles);
-      row_values(r, true, angles, x);
-      fetch(g + 1, r);
-      if (!head_ok || !ch.live) continue;
-      uint8_t* d = dst + static_cast<int64_t>(row) * a.cache_stride[2];
-      if (row >= lo && row < hi) {
-        *reinterpret_cast<uint2*>(d + 8 * ch.c0) = b8_code8<kFmt>(x, s1, r1);
-        *reinterpret_cast<uint2*>(d + 8 * ch.c1) = b8_code8<kFmt>(x + 8, s1, r1);
-      } else if (row < lo && s1 != s0) {  // rows that were there, under a scale that grew
-        uint2* d0 = reinterpret_cast<uint2*>(d + 8 * ch.c0);
-        uint2* d1 = reinterpret_cast<uint2*>(d + 8 * ch.c1);
+      uint2* d0 = reinterpret_cast<uint2*>(dst + r * dst_step + 8 * ch.c0);
+      uint2* d1 = reinterpret_cast<uint2*>(dst + r * dst_step + 8 * ch.c1);
+      if (head_ok && ch.live && is_new(r)) {
+        float x[16];
+        if constexpr (kIsK) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x + 4 * i) = s_val[(4 * r + i) * kThreads];
+        } else {
+          unpack8<BF16>(s_raw[(2 * r) * kThreads], x);
+          unpack8<BF16>(s_raw[(2 * r + 1) * kThreads], x + 8);
+          fetch(g + 1, r);
+        }
+        *d0 = b8_code8<kFmt>(x, s1, r1);
+        *d1 = b8_code8<kFmt>(x + 8, s1, r1);
+      } else if (head_ok && ch.live && row_a + r * row_step < lo && s1 != s0) {  // rows that were there, under a scale that grew
         const uint2 y0 = *d0, y1 = *d1;
         *d0 = b8_recode8<kFmt>(y0, s0, s1, r1);
         *d1 = b8_recode8<kFmt>(y1, s0, s1, r1);
       }
     }
-    cp_async_commit();
+    if (!kIsK) cp_async_commit();
     // one lane of the head's group
     if (head_ok && t == 0 && row_a == 0 && (lo == 0 || s1 != s0)) scales[static_cast<int64_t>(h) * a.scale_stride[1]] = s1;
   }
 }
 
-// Blocks of threads: units of k, then of v; behind them the query rows.
+// Units of k and of v, which take more arithmetic than bandwidth, spread evenly among the blocks that rewrite q, which take more bandwidth.
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const NormRopeArgs a) {
   extern __shared__ __align__(16) float s_dyn[];
@@ -671,12 +686,13 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
   grid_launch_dependents();
   grid_dependency_wait();
   const unsigned per = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch) * static_cast<unsigned>(a.kv_slices);  // blocks of k, and of v
-  if (blockIdx.x < 2 * per) {
-    const bool is_k = blockIdx.x < per;
-    const unsigned i = is_k ? blockIdx.x : blockIdx.x - per;
-    block_role<TPR, BF16, kNeox, kFmt>(a, i / static_cast<unsigned>(a.kv_slices), is_k, i % static_cast<unsigned>(a.kv_slices), static_cast<unsigned>(a.kv_slices), s_dyn, s_max);
+  const unsigned before = static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x) * (2 * per) / gridDim.x);   // units before this block
+  if (static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x + 1) * (2 * per) / gridDim.x) != before) {
+    const unsigned slices = static_cast<unsigned>(a.kv_slices), i = before >> 1;
+    if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false>(a, i / slices, i % slices, slices, s_dyn, s_max);
+    else block_role<TPR, BF16, kNeox, kFmt, true>(a, i / slices, i % slices, slices, s_dyn, s_max);
   } else {
-    rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - 2 * per) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
+    rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
                                              reinterpret_cast<uint4*>(s_dyn));
   }
 }
@@ -774,9 +790,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   a.kv_slices = static_cast<int>(kv_slices);
   const long long blocks = 2 * units * kv_slices + (a.q != nullptr ? row_blocks : 0);
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  // angles between rows, 1 / rms, raw rows
-  size_t smem = 2 * kMaxPairs * sizeof(float) + static_cast<size_t>(blk) * abreast * 4 +
-                static_cast<size_t>((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads) * 32;
+  size_t smem = blocks_smem((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads, true);
   if (a.q != nullptr && smem < static_cast<size_t>(rows_smem(kThreads))) smem = rows_smem(kThreads);
   const unsigned nb = static_cast<unsigned>(blocks);
   if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kE4M3, a, nb, smem, stream);
