@@ -84,12 +84,19 @@ struct Chunks {
   }
 };
 
-// cos and sin of pair i at a position
-__device__ __forceinline__ float2 angle_of(const NormRopeArgs& a, int pos, int i) {
-  const uint64_t turns = static_cast<uint64_t>(static_cast<int64_t>(pos)) * a.turns[i];
+// cos and sin of pair i at a position.  The table is read from shared memory: in the kernel's arguments, lanes that want
+// different entries would be served one after another.
+__device__ __forceinline__ float2 angle_of(const uint64_t* s_turns, int pos, int i) {
+  const uint64_t turns = static_cast<uint64_t>(static_cast<int64_t>(pos)) * s_turns[i];
   float s, c;
   sincospif(static_cast<float>(static_cast<int32_t>(turns >> 32)) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31: half turns
   return make_float2(c, s);
+}
+
+template <int kT>
+__device__ __forceinline__ void copy_turns(const NormRopeArgs& a, uint64_t* s_turns) {
+  for (int u = static_cast<int>(threadIdx.x); u < kMaxPairs; u += kT) s_turns[u] = a.turns[u];
+  __syncthreads();
 }
 
 // 16 weights of a lane's chunks, fp32; `w` points to a head's row of them
@@ -222,14 +229,14 @@ __device__ __forceinline__ void load_angles(const float* cosines, const float* s
 
 // The same computed by a warp whose row groups all work for one token: each group takes its share of a lane's eight angles.
 template <int TPR, bool kNeox>
-__device__ __forceinline__ void warp_angles(const NormRopeArgs& a, int pos, const Chunks<kNeox>& ch, int t, int group, Angles& g) {
+__device__ __forceinline__ void warp_angles(const uint64_t* s_turns, int pos, const Chunks<kNeox>& ch, int t, int group, Angles& g) {
   constexpr int kShare = 8 / (32 / TPR);  // angles per group: 1, 2 or 4
   float2 mine[kShare];
 #pragma unroll
   for (int u = 0; u < kShare; ++u) {
     const int p = group * kShare + u;
     const int i = p < 4 ? ch.i0 + p : ch.i1 + p - 4;
-    mine[u] = angle_of(a, pos, min(i, kMaxPairs - 1));  // (lanes and pairs beyond rotary_dim: some angle that nobody uses)
+    mine[u] = angle_of(s_turns, pos, min(i, kMaxPairs - 1));  // (lanes and pairs beyond rotary_dim: some angle that nobody uses)
   }
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
@@ -291,7 +298,7 @@ struct Cursor {  // of one row group: its two rows of a step
 };
 
 template <int TPR, bool BF16, bool kNeox, int kFmt, int kT>
-__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, unsigned slices, int n_k, int n_v, uint4* s_rows) {
+__device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, unsigned slices, int n_k, int n_v, const uint64_t* s_turns, uint4* s_rows) {
   constexpr int kSide = 32 / TPR;  // row groups of a warp
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 31;
@@ -351,7 +358,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   bool cache_ok = false;
   if (a.k_cache != nullptr && s1 > q_steps) cache_ok = locate(a, b, pos, lane == 0, outer, crow);
   Angles angles = {};
-  if (s0 < q_steps + k_steps && a.rotary_dim > 0) warp_angles<TPR, kNeox>(a, pos, ch, t, group, angles);
+  if (s0 < q_steps + k_steps && a.rotary_dim > 0) warp_angles<TPR, kNeox>(s_turns, pos, ch, t, group, angles);
   Pairs weights = {};
   int weights_of = -1;  // kind
   const int w_bytes = a.w_kind == 2 ? 4 : 2;
@@ -481,10 +488,12 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const NormRopeArgs a) {
   __shared__ __align__(16) uint4 s_rows[rows_smem(kRowThreads) / sizeof(uint4)];
+  __shared__ uint64_t s_turns[kMaxPairs];
   grid_launch_dependents();
+  copy_turns<kRowThreads>(a, s_turns);
   grid_dependency_wait();
   rows_role<TPR, BF16, kNeox, kFmt, kRowThreads>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
-                                                 a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_rows);
+                                                 a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_turns, s_rows);
 }
 
 // ---- blocks of an 8-bit cache: k and v of calls with several tokens per sequence ----
@@ -516,7 +525,7 @@ __device__ __forceinline__ float raw_amax(const uint4& p, const uint4& q) {
 }
 
 template <int TPR, bool BF16, bool kNeox, int kFmt, bool kIsK>
-__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, unsigned slice, unsigned slices, float* smem, float* s_max) {
+__device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, unsigned slice, unsigned slices, const uint64_t* s_turns, float* smem, float* s_max) {
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int blk = 1 << a.log_block;
@@ -567,7 +576,7 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   if (kIsK && pairs > 0) {
     if (rows > 1) {
       for (int u = tid; u < pairs; u += kThreads) {
-        const float2 cs = angle_of(a, row_step, u);
+        const float2 cs = angle_of(s_turns, row_step, u);
         s_cos[u] = cs.x;
         s_sin[u] = cs.y;
       }
@@ -576,7 +585,7 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       if (p < 4 ? ch.rot0 : ch.rot1) {
-        const float2 cs = angle_of(a, base + row_a, p < 4 ? ch.i0 + p : ch.i1 + p - 4);
+        const float2 cs = angle_of(s_turns, base + row_a, p < 4 ? ch.i0 + p : ch.i1 + p - 4);
         (p & 1 ? first.c[p / 2].y : first.c[p / 2].x) = cs.x;
         (p & 1 ? first.s[p / 2].y : first.s[p / 2].x) = cs.y;
         (p & 1 ? first.n[p / 2].y : first.n[p / 2].x) = -cs.y;
@@ -683,17 +692,19 @@ template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const NormRopeArgs a) {
   extern __shared__ __align__(16) float s_dyn[];
   __shared__ float s_max[2 * kThreads / 32];
+  __shared__ uint64_t s_turns[kMaxPairs];
   grid_launch_dependents();
+  copy_turns<kThreads>(a, s_turns);
   grid_dependency_wait();
   const unsigned per = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.n_touch) * static_cast<unsigned>(a.kv_slices);  // blocks of k, and of v
   const unsigned before = static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x) * (2 * per) / gridDim.x);   // units before this block
   if (static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x + 1) * (2 * per) / gridDim.x) != before) {
     const unsigned slices = static_cast<unsigned>(a.kv_slices), i = before >> 1;
-    if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false>(a, i / slices, i % slices, slices, s_dyn, s_max);
-    else block_role<TPR, BF16, kNeox, kFmt, true>(a, i / slices, i % slices, slices, s_dyn, s_max);
+    if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
+    else block_role<TPR, BF16, kNeox, kFmt, true>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
   } else {
     rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
-                                             reinterpret_cast<uint4*>(s_dyn));
+                                             s_turns, reinterpret_cast<uint4*>(s_dyn));
   }
 }
 
@@ -731,7 +742,7 @@ cudaError_t launch_rows(const NormRopeArgs& a, unsigned blocks, cudaStream_t str
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
   auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt>;
-  if (smem > 47 * 1024) {  // (48 KB with the static part)
+  if (smem > 46 * 1024) {  // (48 KB with the static part)
     // (idempotent, and some hundred nanoseconds beside a call of many tokens)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
