@@ -32,23 +32,28 @@ __device__ __forceinline__ float b8_scale(float amax) {
 // 1 / scale (exact for a power of two), 0 for a block of zeros
 __device__ __forceinline__ float b8_inverse(float s) { return s > 0.f ? __frcp_rn(s) : 0.f; }
 
-// the int8 code nearest to x / s: the product with 1 / s decides unless it lies within its error of a border
-__device__ __forceinline__ uint32_t int8_code(float x, float s, float r) {
-  float t = x * r;
-  t = t == t ? fminf(fmaxf(t, -127.f), 127.f) : 0.f;
-  float k = __fadd_rn(t, 12582912.f);
-  if (fabsf(fabsf(t - __fadd_rn(k, -12582912.f)) - 0.5f) < 6e-5f && s > 0.f) {
-    const float q = __fdiv_rn(x, s);
-    const float n = rintf(q);
-    k = n;
-    if (fabsf(q - n) == 0.5f) {  // a border as far as fp32 can tell: the remainder's sign says on which side
-      const float rem = fmaf(-q, s, x);
-      const bool up = s > 0.f ? rem > 0.f : rem < 0.f;
-      if (rem != 0.f) k = up ? ceilf(q) : floorf(q);
-    }
-    k = __fadd_rn(fminf(fmaxf(k, -127.f), 127.f), 12582912.f);
+// The int8 code nearest to x / s (the exact quotient, ties to even), for values that lie near a border between two codes or are not
+// finite.  q is the rounded quotient: it cannot pass a border, only fall on one, and then the remainder's sign decides.
+__device__ __forceinline__ uint32_t int8_code(float x, float s) {
+  const float q = s > 0.f ? __fdiv_rn(x, s) : 0.f;
+  float n = rintf(q);
+  if (fabsf(q - n) == 0.5f) {
+    const float rem = fmaf(-q, s, x);
+    if (rem != 0.f) n = rem > 0.f ? ceilf(q) : floorf(q);
   }
-  return __float_as_uint(k) & 0xFFu;
+  n = q == q ? fminf(fmaxf(n, -127.f), 127.f) : 0.f;
+  return static_cast<uint32_t>(static_cast<int>(n)) & 0xFFu;
+}
+static __device__ __noinline__ uint2 int8_code8(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float s) {
+  return make_uint2(int8_code(x0, s) | (int8_code(x1, s) << 8) | (int8_code(x2, s) << 16) | (int8_code(x3, s) << 24),
+                    int8_code(x4, s) | (int8_code(x5, s) << 8) | (int8_code(x6, s) << 16) | (int8_code(x7, s) << 24));
+}
+
+// larger of two magnitudes, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
 // two fp32 -> two e4m3 in the low 16 bits (lo in the low byte), saturating
@@ -75,20 +80,30 @@ __device__ __forceinline__ uint32_t int8_to_half2(uint32_t src) {
   return *reinterpret_cast<const uint32_t*>(&q);
 }
 
-// eight values -> eight codes; r = 1 / s
+// eight values -> eight codes; r = 1 / s.  Values of magnitude 127.5 s and above do not occur with int8: the scale follows the largest.
 template <int kFmt>
 __device__ __forceinline__ uint2 b8_code8(const float* x, float s, float r) {
   uint32_t w[2];
+  const float2 r2 = make_float2(r, r);
+  float off = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float* y = x + 4 * i;
+    const float2 u = __fmul2_rn(make_float2(y[0], y[1]), r2), v = __fmul2_rn(make_float2(y[2], y[3]), r2);
     if constexpr (kFmt == kE4M3) {
-      const float2 r2 = make_float2(r, r);
-      const float2 u = __fmul2_rn(make_float2(y[0], y[1]), r2), v = __fmul2_rn(make_float2(y[2], y[3]), r2);
       w[i] = e4m3_pair(u.x, u.y) | (e4m3_pair(v.x, v.y) << 16);
     } else {
-      w[i] = int8_code(y[0], s, r) | (int8_code(y[1], s, r) << 8) | (int8_code(y[2], s, r) << 16) | (int8_code(y[3], s, r) << 24);
+      // adding 1.5 * 2^23 rounds to a whole number, which the low byte of the sum holds in two's complement
+      const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+      const float2 ku = __fadd2_rn(u, magic), kv = __fadd2_rn(v, magic);
+      const float2 du = __ffma2_rn(__fadd2_rn(ku, back), minus, u), dv = __ffma2_rn(__fadd2_rn(kv, back), minus, v);
+      off = max_nan(max_nan(max_nan(off, fabsf(du.x)), max_nan(fabsf(du.y), fabsf(dv.x))), fabsf(dv.y));
+      w[i] = __byte_perm(__byte_perm(__float_as_uint(ku.x), __float_as_uint(ku.y), 0x0040), __byte_perm(__float_as_uint(kv.x), __float_as_uint(kv.y), 0x0040), 0x5410);
     }
+  }
+  if constexpr (kFmt == kInt8) {
+    // the product with 1 / s is off by at most 127 * 1.5 * 2^-23 = 2.3e-5: nearer to a border, or not finite, the quotient decides
+    if (!(off < 0.49994f)) return int8_code8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s);
   }
   return make_uint2(w[0], w[1]);
 }
@@ -127,9 +142,15 @@ __device__ __forceinline__ uint2 b8_recode8(uint2 c, float s0, float s1, float r
   return b8_code8<kFmt>(x, s1, r1);
 }
 
+// the same in memory, for rows that only now and then have to be coded again
+template <int kFmt>
+__device__ __noinline__ void b8_recode_at(uint2* p, float s0, float s1, float r1) {
+  *p = b8_recode8<kFmt>(*p, s0, s1, r1);
+}
+
 // rows [0, n) of a block (row_chunks 16-byte chunks each), coded again by `lanes` threads
 template <int kFmt>
-__device__ __forceinline__ void recode_rows(uint8_t* rows, int64_t row_stride, int n, int row_chunks, float s0, float s1, int lane, int lanes) {
+__device__ __noinline__ void recode_rows(uint8_t* rows, int64_t row_stride, int n, int row_chunks, float s0, float s1, int lane, int lanes) {
   const float r1 = b8_inverse(s1);
   constexpr int kBatch = 4;  // loads in flight
   for (int i0 = lane; i0 < n * row_chunks; i0 += kBatch * lanes) {

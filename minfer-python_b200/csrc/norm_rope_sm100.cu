@@ -524,18 +524,17 @@ __device__ __forceinline__ float raw_amax(const uint4& p, const uint4& q) {
   }
 }
 
-template <int TPR, bool BF16, bool kNeox, int kFmt, bool kIsK>
+template <int TPR, bool BF16, bool kNeox, int kFmt, bool kIsK, int kRows>
 __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit, unsigned slice, unsigned slices, const uint64_t* s_turns, float* smem, float* s_max) {
   const int tid = static_cast<int>(threadIdx.x);
   const int t = tid % TPR, rg = tid / TPR;
   const int blk = 1 << a.log_block;
   const int pairs = a.rotary_dim / 2;
-  const int rows = max(1, (blk * TPR) / kThreads);               // per thread
   const int side = max(1, kThreads / (blk * TPR));               // heads side by side
   float* s_cos = smem;                                           // of the angle between two rows of a thread
   float* s_sin = smem + kMaxPairs;
-  uint4* s_raw = reinterpret_cast<uint4*>(smem + 2 * kMaxPairs) + tid;                    // [rows][2] pieces, kThreads apart
-  float4* s_val = reinterpret_cast<float4*>(smem + 2 * kMaxPairs) + rows * 2 * kThreads + tid;  // [rows][4]: k as it is to be coded
+  uint4* s_raw = reinterpret_cast<uint4*>(smem + 2 * kMaxPairs) + tid;                    // [kRows][2] pieces, kThreads apart
+  float4* s_val = reinterpret_cast<float4*>(smem + 2 * kMaxPairs) + kRows * 2 * kThreads + tid;  // [kRows][4]: k as it is to be coded
   const int b = static_cast<int>(unit / static_cast<unsigned>(a.n_touch)), j = static_cast<int>(unit - static_cast<unsigned>(b) * static_cast<unsigned>(a.n_touch));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int64_t start = a.start != nullptr ? a.start[b] : a.start_pos;
@@ -570,11 +569,12 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
       cp_async_16(s_raw + (2 * r + 1) * kThreads, p + 16 * ch.c1, true);
     }
   };
-  for (int r = 0; r < rows; ++r) fetch(g0, r);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) fetch(g0, r);
   cp_async_commit();
   Angles first = {};
   if (kIsK && pairs > 0) {
-    if (rows > 1) {
+    if (kRows > 1) {
       for (int u = tid; u < pairs; u += kThreads) {
         const float2 cs = angle_of(s_turns, row_step, u);
         s_cos[u] = cs.x;
@@ -607,7 +607,8 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     cp_async_wait<0>();
     float amax = 0.f;
     Angles angles = first;
-    for (int r = 0; r < rows; ++r) {
+#pragma unroll 2
+    for (int r = 0; r < kRows; ++r) {
       uint4 raw0 = make_uint4(0, 0, 0, 0), raw1 = raw0;  // (rows that are not new: zeros)
       if (is_new(r) && ch.live) {
         raw0 = s_raw[(2 * r) * kThreads];
@@ -660,7 +661,8 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
     const float s1 = s0 >= need ? s0 : need;
     const float r1 = b8_inverse(s1);
     uint8_t* dst = cache + static_cast<int64_t>(h) * a.cache_stride[1];
-    for (int r = 0; r < rows; ++r) {
+#pragma unroll 2
+    for (int r = 0; r < kRows; ++r) {
       uint2* d0 = reinterpret_cast<uint2*>(dst + r * dst_step + 8 * ch.c0);
       uint2* d1 = reinterpret_cast<uint2*>(dst + r * dst_step + 8 * ch.c1);
       if (head_ok && ch.live && is_new(r)) {
@@ -676,9 +678,8 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
         *d0 = b8_code8<kFmt>(x, s1, r1);
         *d1 = b8_code8<kFmt>(x + 8, s1, r1);
       } else if (head_ok && ch.live && row_a + r * row_step < lo && s1 != s0) {  // rows that were there, under a scale that grew
-        const uint2 y0 = *d0, y1 = *d1;
-        *d0 = b8_recode8<kFmt>(y0, s0, s1, r1);
-        *d1 = b8_recode8<kFmt>(y1, s0, s1, r1);
+        b8_recode_at<kFmt>(d0, s0, s1, r1);
+        b8_recode_at<kFmt>(d1, s0, s1, r1);
       }
     }
     if (!kIsK) cp_async_commit();
@@ -688,7 +689,7 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
 }
 
 // Units of k and of v, which take more arithmetic than bandwidth, spread evenly among the blocks that rewrite q, which take more bandwidth.
-template <int TPR, bool BF16, bool kNeox, int kFmt>
+template <int TPR, bool BF16, bool kNeox, int kFmt, int kRows>
 __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const NormRopeArgs a) {
   extern __shared__ __align__(16) float s_dyn[];
   __shared__ float s_max[2 * kThreads / 32];
@@ -700,8 +701,8 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
   const unsigned before = static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x) * (2 * per) / gridDim.x);   // units before this block
   if (static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x + 1) * (2 * per) / gridDim.x) != before) {
     const unsigned slices = static_cast<unsigned>(a.kv_slices), i = before >> 1;
-    if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
-    else block_role<TPR, BF16, kNeox, kFmt, true>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
+    if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
+    else block_role<TPR, BF16, kNeox, kFmt, true, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
   } else {
     rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
                                              s_turns, reinterpret_cast<uint4*>(s_dyn));
@@ -739,9 +740,9 @@ cudaError_t launch_rows(const NormRopeArgs& a, unsigned blocks, cudaStream_t str
   return cudaLaunchKernelEx(&at.cfg, norm_rope_rows_kernel<TPR, BF16, kNeox, kFmt>, a);
 }
 
-template <int TPR, bool BF16, bool kNeox, int kFmt>
-cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
-  auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt>;
+template <int TPR, bool BF16, bool kNeox, int kFmt, int kRows>
+cudaError_t launch_blocks_rows(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
+  auto* kernel = norm_rope_blocks_kernel<TPR, BF16, kNeox, kFmt, kRows>;
   if (smem > 46 * 1024) {  // (48 KB with the static part)
     // (idempotent, and some hundred nanoseconds beside a call of many tokens)
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -752,6 +753,15 @@ cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, c
   at.cfg.blockDim = dim3(kThreads);
   at.cfg.dynamicSmemBytes = smem;
   return cudaLaunchKernelEx(&at.cfg, kernel, a);
+}
+
+template <int TPR, bool BF16, bool kNeox, int kFmt>
+cudaError_t launch_blocks(const NormRopeArgs& a, unsigned blocks, size_t smem, cudaStream_t stream) {
+  const int lanes = TPR << a.log_block;
+  if (lanes <= kThreads) return launch_blocks_rows<TPR, BF16, kNeox, kFmt, 1>(a, blocks, smem, stream);
+  if (lanes == 2 * kThreads) return launch_blocks_rows<TPR, BF16, kNeox, kFmt, 2>(a, blocks, smem, stream);
+  if constexpr (TPR == 8) return launch_blocks_rows<TPR, BF16, kNeox, kFmt, 4>(a, blocks, smem, stream);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
