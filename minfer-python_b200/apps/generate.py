@@ -9,11 +9,16 @@ of shape [batch, n_kv_heads, max_seq_len, head_dim] (core.py:105-127).
 Projections, norms and the FFN are library calls (torch / cuBLAS): they are outside this
 package's scope.  Attention is this package: `rope_kv_append` rotates q/k and appends k/v to
 the cache in one pass, `flash_attn_causal` does the prompt, `flash_attn_decode` every generated
-token.  Weights are random N(0, 0.02) — there is no checkpoint to load here.
+token.  With `qk_norm` every q and k head is RMS-normed before its rotation (`qk_norm_rope_kv_append`);
+with `kv_cache` "e4m3" or "int8" the caches hold 8-bit codes and a scale per block of `kv_block`
+tokens and head (`rope_kv_append_b8`), a prompt attends to what `kv_read_b8` reads back, and
+`flash_attn_decode_b8` does the generated tokens.  Weights are random N(0, 0.02) — there is no
+checkpoint to load here.
 
     python apps/generate.py                         # Llama-3.2-1B shape, 8 prompts x 512, 128 new tokens
     python apps/generate.py --layers 4 --hidden 512 --heads 8 --kv-heads 2 --ffn 1024 --vocab 1000 \
         --batch 2 --prompt-len 64 --new-tokens 8
+    python apps/generate.py --qk-norm --kv-cache e4m3 --cuda-graph
 """
 from __future__ import annotations
 
@@ -43,6 +48,9 @@ class Shape:
     rope_theta: float = 500000.0
     rope_style: int = 0          # 0 interleaved pairs (the reference's il_rope), 1 neox halves
     eps: float = 1e-5
+    qk_norm: bool = False        # RMS norm of every q and k head before the rotation
+    kv_cache: str = "16bit"      # or "e4m3" / "int8": 8-bit codes, a scale per block of tokens and head
+    kv_block: int = 64           # tokens per scale
 
 
 class Decoder:
@@ -67,6 +75,7 @@ class Decoder:
         self.lm_head = w(s.vocab, s.hidden)
         self.final_norm = torch.ones(s.hidden, dtype=dtype, device=self.dev)
         self.layers = []
+        cache_dtype = {"16bit": dtype, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}[s.kv_cache]
         for _ in range(s.layers):
             self.layers.append(dict(
                 attn_norm=torch.ones(s.hidden, dtype=dtype, device=self.dev),
@@ -75,9 +84,16 @@ class Decoder:
                 ffn_norm=torch.ones(s.hidden, dtype=dtype, device=self.dev),
                 w_gate_up=w(2 * s.ffn, s.hidden),
                 w_down=w(s.hidden, s.ffn),
-                k_cache=torch.zeros(batch, s.kv_heads, max_len, s.head_dim, dtype=dtype, device=self.dev),
-                v_cache=torch.zeros(batch, s.kv_heads, max_len, s.head_dim, dtype=dtype, device=self.dev),
+                k_cache=torch.zeros(batch, s.kv_heads, max_len, s.head_dim, dtype=cache_dtype, device=self.dev),
+                v_cache=torch.zeros(batch, s.kv_heads, max_len, s.head_dim, dtype=cache_dtype, device=self.dev),
             ))
+            if s.qk_norm:
+                self.layers[-1].update(q_norm=torch.ones(s.head_dim, dtype=dtype, device=self.dev),
+                                       k_norm=torch.ones(s.head_dim, dtype=dtype, device=self.dev))
+            if s.kv_cache != "16bit":
+                blocks = -(-max_len // s.kv_block)
+                self.layers[-1].update(k_scale=torch.zeros(batch, s.kv_heads, blocks, device=self.dev),
+                                       v_scale=torch.zeros(batch, s.kv_heads, blocks, device=self.dev))
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)  # tokens in the cache per sequence
         self.attn_ms = 0.0
         self._ev = []
@@ -93,14 +109,24 @@ class Decoder:
         if time_it:
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             e0.record()
-        self.kerns.rope_kv_append(s.head_dim, s.rope_theta, s.rope_style, q, k, v, lay["k_cache"], lay["v_cache"],
-                                  self.lens)
+        turn, caches = (s.head_dim, s.rope_theta, s.rope_style), (lay["k_cache"], lay["v_cache"])
+        norms = (lay["q_norm"], lay["k_norm"]) if s.qk_norm else (None, None)
+        if s.kv_cache != "16bit":
+            caches += (lay["k_scale"], lay["v_scale"], s.kv_block)
+            self.kerns.rope_kv_append_b8(*turn, q, k, v, *caches, self.lens, *norms, s.eps)
+        elif s.qk_norm:
+            self.kerns.qk_norm_rope_kv_append(*turn, s.eps, q, k, v, *norms, *caches, self.lens)
+        else:
+            self.kerns.rope_kv_append(*turn, q, k, v, *caches, self.lens)
         if L > 1:   # prompt: causal attention over the rows just written (the cache starts empty)
-            self.kerns.flash_attn_causal(q.transpose(1, 2), lay["k_cache"][:, :, :L], lay["v_cache"][:, :, :L],
-                                         out.transpose(1, 2))
+            keys, values = lay["k_cache"][:, :, :L], lay["v_cache"][:, :, :L]
+            if s.kv_cache != "16bit":
+                keys, values = (torch.empty(B, s.kv_heads, L, s.head_dim, dtype=self.dtype, device=self.dev) for _ in range(2))
+                self.kerns.kv_read_b8(*caches, self.lens + L, keys, values)
+            self.kerns.flash_attn_causal(q.transpose(1, 2), keys, values, out.transpose(1, 2))
         else:       # one new token per sequence over lens + 1 cached keys
-            self.kerns.flash_attn_decode(q.transpose(1, 2), lay["k_cache"], lay["v_cache"], self._lens_plus,
-                                         out.transpose(1, 2))
+            decode = self.kerns.flash_attn_decode if s.kv_cache == "16bit" else self.kerns.flash_attn_decode_b8
+            decode(q.transpose(1, 2), *caches, self._lens_plus, out.transpose(1, 2))
         if time_it:
             e1.record()
             self._ev.append((e0, e1))
@@ -200,6 +226,9 @@ if __name__ == "__main__":
     ap.add_argument("--vocab", type=int, default=128256)
     ap.add_argument("--rope-theta", type=float, default=500000.0)
     ap.add_argument("--rope-style", type=int, choices=[0, 1], default=0)
+    ap.add_argument("--qk-norm", action="store_true", help="RMS norm of every q and k head")
+    ap.add_argument("--kv-cache", choices=["16bit", "e4m3", "int8"], default="16bit")
+    ap.add_argument("--kv-block", type=int, choices=[16, 32, 64, 128], default=64, help="tokens per scale of an 8-bit cache")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--prompt-len", type=int, default=512)
     ap.add_argument("--new-tokens", type=int, default=128)
@@ -208,7 +237,7 @@ if __name__ == "__main__":
     ap.add_argument("--cuda-graph", action="store_true", help="replay the decode step from a CUDA graph")
     args = ap.parse_args()
     shape = Shape(args.layers, args.hidden, args.heads, args.kv_heads, args.head_dim, args.ffn, args.vocab,
-                  args.rope_theta, args.rope_style)
+                  args.rope_theta, args.rope_style, qk_norm=args.qk_norm, kv_cache=args.kv_cache, kv_block=args.kv_block)
     model = Decoder(shape, args.batch, args.prompt_len + args.new_tokens)
     g = torch.Generator().manual_seed(args.seed)
     prompts = torch.randint(0, args.vocab, (args.batch, args.prompt_len), generator=g).cuda()

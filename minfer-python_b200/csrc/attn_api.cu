@@ -209,28 +209,37 @@ bool table_ok(const int32_t* table, int32_t page_size, int32_t table_stride, int
   return static_cast<int64_t>(page_size) * table_stride >= max_len;
 }
 
-// Blocks (one cluster) per (sequence, kv head) of a decode call over a b8 cache.
+// Blocks (one cluster) per (sequence, kv head) of a decode call over a b8 cache.  As for the other caches the rule knows the padded length only.
+// Measured over 460 shapes (1-2048 pairs of a sequence and a kv head, 64-262144 keys, all of them visible or evenly spread from a
+// sixteenth up; e4m3 and int8, groups of 4, cold caches, back to back in a graph), times in us for 1 / 2 / 4 / 8 / 16 blocks:
+//   one wave (three blocks per SM at head_dim 128, four at 64) for short blocks: 64 pairs of 1024 keys 10 / 11 / 8.4 / 11 / 16;
+//   two of them from 1024 (512) keys per block, 7/3 from 2048, where the tail of a ragged batch costs more than a block's 3 us:
+//   192 pairs of 512-8192 75 / 51 / 41 / 50 / 78.
+//   16 blocks want eight free SMs of one processing cluster: up to 12 (24) pairs, or 48 of long sequences (32 pairs of 2048-32768 32, with
+//   8 blocks 46).
+// Over those shapes the choice costs 2.6 % (head_dim 64: 4.8 %) more than the best of the five, 36 % at worst (384 pairs of 1024-16384, D=64).
 int decode_b8_parts(int64_t batch, int64_t n_kv_heads, int64_t max_len, int64_t head_dim) {
   const int64_t pairs = batch * n_kv_heads;
-  const int64_t wave = 2 * 148;
+  const bool wide = head_dim == 128;
   int parts = 1;
   while (parts < 16 && max_len >= 64 * parts * 2) {
     const int next = parts * 2;
-    const int64_t block_bytes = max_len / next * head_dim;
-    const int64_t limit = block_bytes >= (512 << 10) ? wave * 7 / 2 : block_bytes >= (256 << 10) ? wave * 2 : wave;
+    const int64_t keys = max_len / next;
+    const int64_t limit = keys >= 2048 ? 7 * 148 : keys >= (wide ? 1024 : 512) ? 6 * 148 : (wide ? 3 : 4) * 148;
     if (pairs * next > limit) break;
-    if (next == 16 && pairs > 12) break;
+    if (next == 16 && pairs > (wide ? 12 : 24) && !(pairs <= 48 && keys >= (wide ? 2048 : 512))) break;
     parts = next;
   }
   return parts;
 }
 
-// Keys per block of the form that leaves partial outputs in the workspace, 0 where clusters are used.
-int32_t decode_b8_chunk(int64_t batch, int64_t n_kv_heads, int64_t max_len) {
-  (void)batch;
-  (void)n_kv_heads;
-  (void)max_len;
-  return 0;
+// Blocks per pair where a cluster's 16 leave SMs idle and there is that much to read: partial outputs through the workspace and a second,
+// small launch that adds them up; 0: clusters.  Clusters / this: 1 pair of 65536 keys 28 / 28, of 131072 51 / 39, of 262144 98 / 44; 8 pairs of
+// 16384 17 / 16, of 131072 77 / 57; 16 pairs of 8192 14.0 / 13.3, of 32768 38 / 30; 24 of 32768 45 / 41; 32 of 8192 16.3 / 17.0.
+int decode_b8_split(int64_t batch, int64_t n_kv_heads, int64_t max_len, int64_t head_dim) {
+  const int64_t pairs = batch * n_kv_heads;
+  if (pairs > 24 || pairs * max_len * head_dim < (int64_t{16} << 20)) return 0;
+  return static_cast<int>(2 * 148 / pairs);
 }
 
 }  // namespace
@@ -629,9 +638,7 @@ int minfer_attn_norm_rope_append(const MinferNormRopeParams* p, void* stream) {
 
 size_t minfer_attn_decode_b8_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t max_len, int32_t head_dim) {
   if (batch <= 0 || n_heads <= 0 || n_kv_heads <= 0 || max_len <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  const int32_t chunk = decode_b8_chunk(batch, n_kv_heads, max_len);
-  if (chunk == 0) return 0;
-  return static_cast<size_t>(batch) * n_heads * ((static_cast<size_t>(max_len) + chunk - 1) / chunk) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
+  return static_cast<size_t>(batch) * n_heads * decode_b8_split(batch, n_kv_heads, max_len, head_dim) * (static_cast<size_t>(head_dim) + 2) * sizeof(float);
 }
 
 int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* p, void* stream) {
@@ -674,14 +681,15 @@ int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* p, void* stream) {
   a.group = group;
   const int64_t pairs = static_cast<int64_t>(p->batch) * p->n_kv_heads;
   if (need > 0 && p->workspace != nullptr) {
-    a.chunk = decode_b8_chunk(p->batch, p->n_kv_heads, p->max_len);
-    a.n_split = (p->max_len + a.chunk - 1) / a.chunk;
+    a.n_split = decode_b8_split(p->batch, p->n_kv_heads, p->max_len, p->head_dim);
     a.part_o = static_cast<float*>(p->workspace);
     a.part_ml = a.part_o + static_cast<size_t>(p->batch) * p->n_heads * a.n_split * p->head_dim;
   } else {
     a.n_split = decode_b8_parts(p->batch, p->n_kv_heads, p->max_len, p->head_dim);
     a.by_length = (p->batch > 1 && p->batch <= 256 && pairs * a.n_split > 2 * 148 && decode_is_large(pairs, p->max_len, p->head_dim)) ? 1 : 0;
   }
+  // deeper rings where the call has no more blocks than two per SM (one at head_dim 64): 128 pairs of 2048 keys 16 / 19 us
+  a.deep = pairs * a.n_split <= (a.part_o != nullptr || p->head_dim == 128 ? 2 : 1) * 148 ? 1 : 0;
   for (int i = 0; i < 2; ++i) {
     a.q_stride[i] = p->q_stride[i];
     a.out_stride[i] = p->out_stride[i];

@@ -135,6 +135,7 @@ struct DecodeB8Args : DecodeArgs {
   const float* v_scale;
   int64_t scale_stride[2];  // elements: batch (or page), head
   int32_t log_block;        // log2 of the tokens per block
+  int32_t deep;             // the deeper rings: two thread blocks per SM, not three
 };
 
 cudaError_t launch_decode_b8(const DecodeB8Args& a, int head_dim, bool bf16, bool int8, cudaStream_t stream);

@@ -31,18 +31,14 @@ namespace minfer_attn {
 
 namespace {
 
-#ifndef MINFER_ATTN_B8_STAGES
-#define MINFER_ATTN_B8_STAGES 6
-#endif
-#ifndef MINFER_ATTN_B8_CTAS
-#define MINFER_ATTN_B8_CTAS 2
-#endif
+constexpr int kShallow = 4;  // stages of a ring where three blocks share an SM
+constexpr int kDeep = 6;     // and where no more than two do
 constexpr float kWeightLog = 14.f;   // log2 of the largest weight, as stored
 constexpr int kLeastScaleLog = -90;  // a scale's log2, as far as the reference m follows it
 
-template <int D, int NT>
+template <int D, int NT, int kSt>
 struct LayoutB8 {
-  static constexpr int kStages = MINFER_ATTN_B8_STAGES;
+  static constexpr int kStages = kSt;
   static constexpr int kTileBytes = kTileKeys * D;
   static constexpr int kStageBytes = 2 * kTileBytes + 16;  // K, V, the tile's scales (two floats)
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -80,15 +76,222 @@ __device__ __forceinline__ void word_to_half(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-template <int D, bool BF16, bool I8, bool Paged, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? MINFER_ATTN_B8_CTAS : 2) decode_b8_kernel(const DecodeB8Args a) {
-  using L = LayoutB8<D, NT>;
-  constexpr int kSt = L::kStages;
+// What a warp keeps of one (sequence, kv head): the queries, and the running output, reference and sum.
+template <int D, int NT>
+struct WarpState {
+  uint32_t qf[NT][D / 16][2];  // Q^T fragments (B operand), fp16
+  float qs[NT][2];             // per column (heads 2 tq, 2 tq + 1): softmax scale * log2(e) * the power of two taken out of the queries
+  float oacc[NT][D / 16][4];   // O^T
+  float m_ref[NT][2], l_run[NT][2];  // reference maximum (log2 domain), this lane's share of the row sum
+};
+
+// Queries of kv head kvh of sequence b; step (u, i) of the first product holds dimensions 16 (2 tq + u) + 4 i + {0 .. 3} of lane tq
+// (head_dim 64: 16 tq + 4 i).  The running values start anew.
+template <int D, bool BF16, int NT>
+__device__ __forceinline__ void start_pair(const DecodeB8Args& a, int b, int kvh, int lane, WarpState<D, NT>& w) {
+  const int g0 = lane >> 2, tq = lane & 3;
+  constexpr int kU = D / 64;
+  const uint8_t* qb = reinterpret_cast<const uint8_t*>(a.q) + 2 * static_cast<int64_t>(b) * a.q_stride[0];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int g = g0 + 8 * n;
+    const bool live = g < a.group;
+    const uint8_t* qp = qb + 2 * static_cast<int64_t>(kvh * a.group + (live ? g : 0)) * a.q_stride[1];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 x = *reinterpret_cast<const uint4*>(qp + 32 * (kU * tq + u) + 16 * h);
+        w.qf[n][4 * u + 2 * h][0] = live ? x.x : 0u;
+        w.qf[n][4 * u + 2 * h][1] = live ? x.y : 0u;
+        w.qf[n][4 * u + 2 * h + 1][0] = live ? x.z : 0u;
+        w.qf[n][4 * u + 2 * h + 1][1] = live ? x.w : 0u;
+      }
+    }
+    float back = 1.f;  // of head g
+    if constexpr (BF16) {
+      uint32_t top = 0;  // largest magnitude, as bits
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top = max(top, max(w.qf[n][s][e] & 0x7FFFu, (w.qf[n][s][e] >> 16) & 0x7FFFu));
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+      // the largest becomes 2^14 .. 2^15; exponents kept so that neither factor leaves fp32's range
+      const int e = max(-110, min(110, 127 + 14 - static_cast<int>(top >> 7)));
+      const float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      back = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int e2 = 0; e2 < 2; ++e2)
+          w.qf[n][s][e2] = pack2<false>(__uint_as_float(w.qf[n][s][e2] << 16) * f, __uint_as_float(w.qf[n][s][e2] & 0xFFFF0000u) * f);
+    }
+    w.qs[n][0] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq);
+    w.qs[n][1] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq + 4);
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) w.oacc[n][m][0] = w.oacc[n][m][1] = w.oacc[n][m][2] = w.oacc[n][m][3] = 0.f;
+    w.m_ref[n][0] = w.m_ref[n][1] = -INFINITY;
+    w.l_run[n][0] = w.l_run[n][1] = 0.f;
+  }
+}
+
+// One tile of 16 keys that lies in a stage of the ring; the first `live` of them count.
+template <int D, bool I8, int NT>
+__device__ __forceinline__ void process_tile(const uint8_t* tk, int live, int lane, WarpState<D, NT>& w) {
+  constexpr int kTileBytes = kTileKeys * D;
+  constexpr int kU = D / 64;
+  const int g0 = lane >> 2, tq = lane & 3;
+  const uint8_t* tv = tk + kTileBytes;
+  const float2 scales = *reinterpret_cast<const float2*>(tk + 2 * kTileBytes);
+  // ---- S^T[16 keys x 8 heads] = K Q^T (two accumulators: half the chain of dependent MMAs) ----
+  float s[NT][4], s2[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint4 x = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0, kU * tq + u));
+    const uint4 y = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0 + 8, kU * tq + u));
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t kf[4];
+      word_to_half<I8>(xw[j], kf[0], kf[2]);
+      word_to_half<I8>(yw[j], kf[1], kf[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_16816<false>((j & 1) ? s2[n] : s[n], kf, w.qf[n][4 * u + j][0], w.qf[n][4 * u + j][1]);
+    }
+  }
+  // ---- online softmax: x = t - m; 2^x times the scale has to stay within 2^14; a tile in which it does needs no reduction over
+  // the lanes ----
+  const bool dead0 = g0 >= live, dead1 = g0 + 8 >= live;
+  const float room = kWeightLog - static_cast<float>(max(static_cast<int>((__float_as_uint(scales.y) + 0x7FFFFFu) >> 23) - 127, kLeastScaleLog));
+  float x[NT][4];
+  bool move = false;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float f0 = w.qs[n][0] * scales.x, f1 = w.qs[n][1] * scales.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[n][e] = (s[n][e] + s2[n][e]) * ((e & 1) ? f1 : f0);
+      if (e < 2 ? dead0 : dead1) s[n][e] = -INFINITY;
+      x[n][e] = s[n][e] - w.m_ref[n][e & 1];  // +inf before the first tile (-inf - -inf: NaN, which moves nothing)
+    }
+    move |= fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) > room;
+  }
+  if (__any_sync(0xFFFFFFFFu, move)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = fmaxf(s[n][h], s[n][2 + h]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+        const float m_new = fmaxf(w.m_ref[n][h], mx - room);
+        alpha[h] = ex2_approx(w.m_ref[n][h] - m_new);
+        w.m_ref[n][h] = m_new;
+        w.l_run[n][h] *= alpha[h];
+      }
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) {
+        w.oacc[n][m][0] *= alpha[0];
+        w.oacc[n][m][1] *= alpha[1];
+        w.oacc[n][m][2] *= alpha[0];
+        w.oacc[n][m][3] *= alpha[1];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] = s[n][e] - w.m_ref[n][e & 1];
+    }
+  }
+  uint32_t pb[NT][2];  // P^T fragments (B operand): keys 2 tq, 2 tq + 1 (+ 8) of head g0
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[n][e] = ex2_approx(x[n][e]);
+    w.l_run[n][0] += x[n][0] + x[n][2];
+    w.l_run[n][1] += x[n][1] + x[n][3];
+    pb[n][0] = movmatrix_trans(pack2<false>(x[n][0] * scales.y, x[n][1] * scales.y));
+    pb[n][1] = movmatrix_trans(pack2<false>(x[n][2] * scales.y, x[n][3] * scales.y));
+  }
+
+  // ---- O^T[D x 8 heads] += V^T P^T: lane (g0, tq) reads D / 8 dimensions of its four keys and interleaves the keys pairwise; rows g0 and
+  // g0 + 8 of 16-row tile m are dimensions (D / 8) g0 + 2 m and + 1 ----
+  constexpr int kVWords = D / 32;
+  uint32_t vw[4][kVWords];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = 2 * tq + (r & 1) + 8 * (r >> 1);
+    if constexpr (D == 128) {
+      const uint4 y = *reinterpret_cast<const uint4*>(tv + chunk_at<D>(row, g0));
+      vw[r][0] = y.x;
+      vw[r][1] = y.y;
+      vw[r][2] = y.z;
+      vw[r][3] = y.w;
+    } else {
+      const uint2 y = *reinterpret_cast<const uint2*>(tv + chunk_at<D>(row, g0 >> 1) + 8 * (g0 & 1));
+      vw[r][0] = y.x;
+      vw[r][1] = y.y;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < D / 16; ++m) {
+    const int j = m >> 1;
+    uint32_t vf[4];
+    word_to_half<I8>(__byte_perm(vw[0][j], vw[1][j], (m & 1) ? 0x7362 : 0x5140), vf[0], vf[1]);
+    word_to_half<I8>(__byte_perm(vw[2][j], vw[3][j], (m & 1) ? 0x7362 : 0x5140), vf[2], vf[3]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma_16816<false>(w.oacc[n][m], vf, pb[n][0], pb[n][1]);
+  }
+}
+
+// Sums the lanes' shares of the row sums; every lane of a column then holds its sum.
+template <int D, int NT>
+__device__ __forceinline__ void finish_pair(WarpState<D, NT>& w) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      w.l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, w.l_run[n][h], 4);
+      w.l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, w.l_run[n][h], 8);
+      w.l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, w.l_run[n][h], 16);
+    }
+}
+
+// head g = 8 n + 2 tq + h of the pair: this lane's D / 8 dimensions, from (D / 8) g0 on, to `row` (a row of D floats)
+template <int D, int NT>
+__device__ __forceinline__ void store_partial(const WarpState<D, NT>& w, int n, int h, float* row, int g0) {
+#pragma unroll
+  for (int m = 0; m < D / 16; m += 2)
+    *reinterpret_cast<float4*>(row + (D / 8) * g0 + 2 * m) = make_float4(w.oacc[n][m][h], w.oacc[n][m][2 + h], w.oacc[n][m + 1][h], w.oacc[n][m + 1][2 + h]);
+}
+
+// Asynchronous copies of one tile into a stage: `k`, `v` point to this lane's chunk of its first row, `live` rows from that row on exist.
+template <int D>
+__device__ __forceinline__ void copy_tile(uint8_t* stage, const uint8_t* k, const uint8_t* v, int64_t load_step, int live, int l_row, int l_chunk,
+                                          const void* safe_k, const void* safe_v) {
+  constexpr int kRowsPerLoad = 32 / (D / 16);  // rows that one instruction of a warp brings
+#pragma unroll
+  for (int t = 0; t < kTileKeys / kRowsPerLoad; ++t) {
+    const bool pred = t * kRowsPerLoad < live;  // rows beyond the sequence are not read and count as zeros
+    const uint32_t at = chunk_at<D>(t * kRowsPerLoad + l_row, l_chunk);
+    cp_async_16(stage + at, pred ? k : safe_k, pred);
+    cp_async_16(stage + kTileKeys * D + at, pred ? v : safe_v, pred);
+    k += load_step;
+    v += load_step;
+  }
+}
+
+template <int D, bool BF16, bool I8, bool Paged, int NT, int kSt>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 && kSt == kShallow ? 3 : 2) decode_b8_kernel(const DecodeB8Args a) {
+  using L = LayoutB8<D, NT, kSt>;
   constexpr int kTileBytes = L::kTileBytes;
   constexpr int kWarpBytes = L::kWarpBytes;
   constexpr int kChunksPerRow = D / 16;
   constexpr int kRowsPerLoad = 32 / kChunksPerRow;           // rows that one instruction of a warp brings
-  constexpr int kLoads = kTileKeys / kRowsPerLoad;
 
   extern __shared__ __align__(128) uint8_t smem[];
 
@@ -123,27 +326,31 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? MINFER_ATTN_B8_CTAS : 2
   } else {
     len = max(0, min(a.lens[b], a.max_len));
   }
-  int c0, c1;
-  if (clustered) {
-    const int nt_seq = (len + kTileKeys - 1) / kTileKeys;
-    c0 = static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part) / static_cast<unsigned>(n_parts)) * kTileKeys;
-    c1 = min(len, static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part + 1) / static_cast<unsigned>(n_parts)) * kTileKeys);
-  } else {
-    c0 = part * a.chunk;
-    if (c0 >= len) return;
-    c1 = min(len, c0 + a.chunk);
-  }
+  // the keys of this block: an even share of the sequence's tiles
+  const int nt_seq = (len + kTileKeys - 1) / kTileKeys;
+  const int c0 = static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part) / static_cast<unsigned>(n_parts)) * kTileKeys;
+  const int c1 = min(len, static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part + 1) / static_cast<unsigned>(n_parts)) * kTileKeys);
   const int nt = c1 > c0 ? (c1 - c0 + kTileKeys - 1) / kTileKeys : 0;
   const int nt_w = (nt > warp) ? (nt - warp + kWarps - 1) / kWarps : 0;
 
   uint8_t* wsm = smem + warp * kWarpBytes;
   const int l_row = lane / kChunksPerRow, l_chunk = lane % kChunksPerRow;
 
-  auto issue_tile = [&](int i) {  // i-th tile of this warp -> stage i % kSt
+  // This lane's first row and chunk of the tile to be fetched next, and the scale that it fetches (lane 0 of k's block, lane 1 of v's).  A contiguous
+  // cache moves on by a fixed step; pages are looked up tile by tile (a tile lies in one).
+  const int64_t lane_off = static_cast<int64_t>(kvh) * a.kv_stride[1] + static_cast<int64_t>(l_row) * a.kv_stride[2] + l_chunk * 16;
+  const int64_t load_step = kRowsPerLoad * a.kv_stride[2];
+  const float* scale_base = (lane == 0 ? a.k_scale : a.v_scale) + static_cast<int64_t>(kvh) * a.scale_stride[1];
+  const int key_w = c0 + warp * kTileKeys;  // first key of this warp
+  int64_t off = lane_off;
+  if constexpr (!Paged) {
+    off += static_cast<int64_t>(b) * a.kv_stride[0] + static_cast<int64_t>(key_w) * a.kv_stride[2];
+    scale_base += static_cast<int64_t>(b) * a.scale_stride[0];
+  }
+  auto issue_tile = [&](int i) {  // i-th tile of this warp -> stage i % kSt; called for i = 0, 1, 2, ...
     if (i < nt_w) {
-      const int key0 = c0 + (warp + i * kWarps) * kTileKeys;
-      int64_t toff = static_cast<int64_t>(kvh) * a.kv_stride[1];
-      int64_t soff = static_cast<int64_t>(kvh) * a.scale_stride[1];
+      const int key0 = key_w + i * (kWarps * kTileKeys);
+      int64_t soff;
       if constexpr (Paged) {
         const int slot = key0 / a.page_size;
         int page = a.block_table[static_cast<size_t>(b) * a.table_stride + slot];
@@ -152,27 +359,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? MINFER_ATTN_B8_CTAS : 2
           page = 0;
         }
         const int row = key0 - slot * a.page_size;
-        toff += static_cast<int64_t>(page) * a.kv_stride[0] + static_cast<int64_t>(row) * a.kv_stride[2];
-        soff += static_cast<int64_t>(page) * a.scale_stride[0] + (row >> a.log_block);
+        off = lane_off + static_cast<int64_t>(page) * a.kv_stride[0] + static_cast<int64_t>(row) * a.kv_stride[2];
+        soff = static_cast<int64_t>(page) * a.scale_stride[0] + (row >> a.log_block);
       } else {
-        toff += static_cast<int64_t>(b) * a.kv_stride[0] + static_cast<int64_t>(key0) * a.kv_stride[2];
-        soff += static_cast<int64_t>(b) * a.scale_stride[0] + (key0 >> a.log_block);
+        soff = key0 >> a.log_block;
       }
       uint8_t* dst_k = wsm + (i % kSt) * L::kStageBytes;
-      uint8_t* dst_v = dst_k + kTileBytes;
-      const uint8_t* src_k = reinterpret_cast<const uint8_t*>(a.k) + toff + l_chunk * 16;
-      const uint8_t* src_v = reinterpret_cast<const uint8_t*>(a.v) + toff + l_chunk * 16;
-      const int live = c1 - key0;
-#pragma unroll
-      for (int t = 0; t < kLoads; ++t) {
-        const int row = t * kRowsPerLoad + l_row;
-        const bool pred = row < live;  // rows beyond the sequence are not read and count as zeros
-        const int64_t off = static_cast<int64_t>(pred ? row : 0) * a.kv_stride[2];
-        const uint32_t at = chunk_at<D>(row, l_chunk);
-        cp_async_16(dst_k + at, src_k + off, pred);
-        cp_async_16(dst_v + at, src_v + off, pred);
-      }
-      if (lane < 2) cp_async_4(dst_k + 2 * kTileBytes + 4 * lane, (lane == 0 ? a.k_scale : a.v_scale) + soff);
+      copy_tile<D>(dst_k, reinterpret_cast<const uint8_t*>(a.k) + off, reinterpret_cast<const uint8_t*>(a.v) + off, load_step, c1 - key0 - l_row, l_row, l_chunk, a.k, a.v);
+      if (lane < 2) cp_async_4(dst_k + 2 * kTileBytes + 4 * lane, scale_base + soff);
+      if constexpr (!Paged) off += (kWarps * kTileKeys) * a.kv_stride[2];
     }
     cp_async_commit();
   };
@@ -181,226 +376,130 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? MINFER_ATTN_B8_CTAS : 2
 #pragma unroll
   for (int s = 0; s < kSt - 1; ++s) issue_tile(s);
 
-  // ---- Q^T fragments (B operand), fp16: step (u, i) holds dimensions 16 (2 tq + u) + 4 i + {0 .. 3} of lane tq (head_dim 64: 16 tq + 4 i) ----
-  const int g0 = lane >> 2;
-  const int tq = lane & 3;
-  constexpr int kU = D / 64;
-  uint32_t qf[NT][D / 16][2];
-  float qs[NT][2];  // per column (heads 2 tq, 2 tq + 1): softmax scale * log2(e) * the power of two taken out of the queries
-  {
-    const uint8_t* qb = reinterpret_cast<const uint8_t*>(a.q) + 2 * static_cast<int64_t>(b) * a.q_stride[0];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int g = g0 + 8 * n;
-      const bool live = g < a.group;
-      const uint8_t* qp = qb + 2 * static_cast<int64_t>(kvh * a.group + (live ? g : 0)) * a.q_stride[1];
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 x = *reinterpret_cast<const uint4*>(qp + 32 * (kU * tq + u) + 16 * h);
-          qf[n][4 * u + 2 * h][0] = live ? x.x : 0u;
-          qf[n][4 * u + 2 * h][1] = live ? x.y : 0u;
-          qf[n][4 * u + 2 * h + 1][0] = live ? x.z : 0u;
-          qf[n][4 * u + 2 * h + 1][1] = live ? x.w : 0u;
-        }
-      }
-      float back = 1.f;  // of head g
-      if constexpr (BF16) {
-        uint32_t top = 0;  // largest magnitude, as bits
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) top = max(top, max(qf[n][s][e] & 0x7FFFu, (qf[n][s][e] >> 16) & 0x7FFFu));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        // the largest becomes 2^14 .. 2^15; exponents kept so that neither factor leaves fp32's range
-        const int e = max(-110, min(110, 127 + 14 - static_cast<int>(top >> 7)));
-        const float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        back = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            qf[n][s][w] = pack2<false>(__uint_as_float(qf[n][s][w] << 16) * f, __uint_as_float(qf[n][s][w] & 0xFFFF0000u) * f);
-      }
-      qs[n][0] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq);
-      qs[n][1] = a.scale_log2 * __shfl_sync(0xFFFFFFFFu, back, 8 * tq + 4);
-    }
-  }
-
-  float oacc[NT][D / 16][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int m = 0; m < D / 16; ++m) oacc[n][m][0] = oacc[n][m][1] = oacc[n][m][2] = oacc[n][m][3] = 0.f;
-  float m_ref[NT][2], l_run[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_ref[n][0] = m_ref[n][1] = -INFINITY;
-    l_run[n][0] = l_run[n][1] = 0.f;
-  }
-
+  WarpState<D, NT> w;
+  start_pair<D, BF16, NT>(a, b, kvh, lane, w);
   for (int i = 0; i < nt_w; ++i) {
     cp_async_wait<kSt - 2>();
     __syncwarp();
     issue_tile(i + kSt - 1);
-
-    const int key0 = c0 + (warp + i * kWarps) * kTileKeys;
-    const uint8_t* tk = wsm + (i % kSt) * L::kStageBytes;
-    const uint8_t* tv = tk + kTileBytes;
-    const float2 scales = *reinterpret_cast<const float2*>(tk + 2 * kTileBytes);
-    // ---- S^T[16 keys x 8 heads] = K Q^T (two accumulators: half the chain of dependent MMAs) ----
-    float s[NT][4], s2[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const uint4 x = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0, kU * tq + u));
-      const uint4 y = *reinterpret_cast<const uint4*>(tk + chunk_at<D>(g0 + 8, kU * tq + u));
-      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t kf[4];
-        word_to_half<I8>(xw[w], kf[0], kf[2]);
-        word_to_half<I8>(yw[w], kf[1], kf[3]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma_16816<false>((w & 1) ? s2[n] : s[n], kf, qf[n][4 * u + w][0], qf[n][4 * u + w][1]);
-      }
-    }
-    // ---- online softmax: x = t - m; 2^x times the scale has to stay within 2^14; a tile in which it does needs no reduction over
-    // the lanes ----
-    const bool partial = key0 + kTileKeys > c1;
-    const bool dead0 = partial && key0 + g0 >= c1, dead1 = partial && key0 + g0 + 8 >= c1;
-    const float room = kWeightLog - static_cast<float>(max(static_cast<int>((__float_as_uint(scales.y) + 0x7FFFFFu) >> 23) - 127, kLeastScaleLog));
-    float x[NT][4];
-    bool move = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float f0 = qs[n][0] * scales.x, f1 = qs[n][1] * scales.x;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[n][e] = (s[n][e] + s2[n][e]) * ((e & 1) ? f1 : f0);
-        if (e < 2 ? dead0 : dead1) s[n][e] = -INFINITY;
-        x[n][e] = s[n][e] - m_ref[n][e & 1];  // +inf before the first tile (-inf - -inf: NaN, which moves nothing)
-      }
-      move |= fmaxf(fmaxf(x[n][0], x[n][1]), fmaxf(x[n][2], x[n][3])) > room;
-    }
-    if (__any_sync(0xFFFFFFFFu, move)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float alpha[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float mx = fmaxf(s[n][h], s[n][2 + h]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
-          const float m_new = fmaxf(m_ref[n][h], mx - room);
-          alpha[h] = ex2_approx(m_ref[n][h] - m_new);
-          m_ref[n][h] = m_new;
-          l_run[n][h] *= alpha[h];
-        }
-#pragma unroll
-        for (int m = 0; m < D / 16; ++m) {
-          oacc[n][m][0] *= alpha[0];
-          oacc[n][m][1] *= alpha[1];
-          oacc[n][m][2] *= alpha[0];
-          oacc[n][m][3] *= alpha[1];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = s[n][e] - m_ref[n][e & 1];
-      }
-    }
-    uint32_t pb[NT][2];  // P^T fragments (B operand): keys 2 tq, 2 tq + 1 (+ 8) of head g0
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[n][e] = ex2_approx(x[n][e]);
-      l_run[n][0] += x[n][0] + x[n][2];
-      l_run[n][1] += x[n][1] + x[n][3];
-      pb[n][0] = movmatrix_trans(pack2<false>(x[n][0] * scales.y, x[n][1] * scales.y));
-      pb[n][1] = movmatrix_trans(pack2<false>(x[n][2] * scales.y, x[n][3] * scales.y));
-    }
-
-    // ---- O^T[D x 8 heads] += V^T P^T: lane (g0, tq) reads D / 8 dimensions of its four keys and interleaves the keys pairwise; rows g0 and
-    // g0 + 8 of 16-row tile m are dimensions (D / 8) g0 + 2 m and + 1 ----
-    constexpr int kVWords = D / 32;
-    uint32_t vw[4][kVWords];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 2 * tq + (r & 1) + 8 * (r >> 1);
-      if constexpr (D == 128) {
-        const uint4 y = *reinterpret_cast<const uint4*>(tv + chunk_at<D>(row, g0));
-        vw[r][0] = y.x;
-        vw[r][1] = y.y;
-        vw[r][2] = y.z;
-        vw[r][3] = y.w;
-      } else {
-        const uint2 y = *reinterpret_cast<const uint2*>(tv + chunk_at<D>(row, g0 >> 1) + 8 * (g0 & 1));
-        vw[r][0] = y.x;
-        vw[r][1] = y.y;
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < D / 16; ++m) {
-      const int w = m >> 1;
-      uint32_t vf[4];
-      word_to_half<I8>(__byte_perm(vw[0][w], vw[1][w], (m & 1) ? 0x7362 : 0x5140), vf[0], vf[1]);
-      word_to_half<I8>(__byte_perm(vw[2][w], vw[3][w], (m & 1) ? 0x7362 : 0x5140), vf[2], vf[3]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mma_16816<false>(oacc[n][m], vf, pb[n][0], pb[n][1]);
-    }
+    process_tile<D, I8, NT>(wsm + (i % kSt) * L::kStageBytes, c1 - key_w - i * (kWarps * kTileKeys), lane, w);
   }
   cp_async_wait<0>();
+  finish_pair<D, NT>(w);
+  __syncthreads();
 
   // ---- this warp's partial output into its part of the ring ----
-  const int group = a.group;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 4);
-      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 8);
-      l_run[n][h] += __shfl_xor_sync(0xFFFFFFFFu, l_run[n][h], 16);
-    }
-  __syncthreads();
-  constexpr int kRow = D + 4;
   float* mo = reinterpret_cast<float*>(wsm);
   float2* wml = reinterpret_cast<float2*>(smem + L::kRingBytes);
+  const int g0 = lane >> 2, tq = lane & 3;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int g = 8 * n + 2 * tq + h;
-      if (g < group) {
-#pragma unroll
-        for (int m = 0; m < D / 16; m += 2)
-          *reinterpret_cast<float4*>(&mo[g * kRow + (D / 8) * g0 + 2 * m]) =
-              make_float4(oacc[n][m][h], oacc[n][m][2 + h], oacc[n][m + 1][h], oacc[n][m + 1][2 + h]);
-        if (g0 == 0) wml[warp * 8 * NT + g] = make_float2(m_ref[n][h], l_run[n][h]);
+      if (g < a.group) {
+        store_partial<D, NT>(w, n, h, mo + g * (D + 4), g0);
+        if (g0 == 0) wml[warp * 8 * NT + g] = make_float2(w.m_ref[n][h], w.l_run[n][h]);
       }
     }
   merge_partials<D, BF16, NT, L, true>(a, smem, arrived, abort_flag, b, kvh, part, n_parts, clustered, tid);
 }
 
-template <int D, bool BF16, bool I8, bool Paged, int NT>
-cudaError_t launch_heads(const DecodeB8Args& a, cudaStream_t stream) {
-  auto* kernel = decode_b8_kernel<D, BF16, I8, Paged, NT>;
-  constexpr int smem = LayoutB8<D, NT>::kBytes;
-  static std::atomic<bool> attr_done[64] = {};  // set-once flags; the attribute calls themselves are idempotent
+// Grid (n_heads, batch), where the blocks of a pair are too many for a cluster: adds up the n_split partial outputs of one head.  A problem of
+// latencies: the maximum, then the weights over all threads, then the outputs over all warps, four loads in flight.
+constexpr int kMergeWarps = 8;
+constexpr int kMaxSplit = 2 * 148;
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(32 * kMergeWarps) decode_b8_merge_kernel(const DecodeB8Args a) {
+  constexpr int kLanes = D / 4, kSide = 32 / kLanes;  // lanes per partial output, outputs side by side in a warp
+  __shared__ float s_w[kMaxSplit];
+  __shared__ __align__(16) float4 s_o[kMergeWarps * kSide][kLanes];
+  __shared__ float s_f[2][kMergeWarps];
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const size_t p0 = (static_cast<size_t>(b) * a.n_heads + h) * a.n_split;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + p0;
+  grid_launch_dependents();
+  grid_dependency_wait();
+  float M = -INFINITY;
+  for (int i = tid; i < a.n_split; i += 32 * kMergeWarps) M = fmaxf(M, ml[i].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+  if (lane == 0) s_f[0][warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < kMergeWarps; ++v) M = fmaxf(M, s_f[0][v]);
+  float l = 0.f;
+  for (int i = tid; i < a.n_split; i += 32 * kMergeWarps) {
+    const float2 x = ml[i];
+    const float f = x.x == -INFINITY ? 0.f : ex2_approx(x.x - M);
+    s_w[i] = f;
+    l += f * x.y;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+  if (lane == 0) s_f[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int v = 0; v < kMergeWarps; ++v) l += s_f[1][v];
+  const int sub = lane / kLanes, t = lane % kLanes;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o) + p0 * kLanes + t;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = warp * kSide + sub; i < a.n_split; i += kMergeWarps * kSide) {
+    const float4 x = po[static_cast<size_t>(i) * kLanes];
+    const float f = s_w[i];
+    o.x += f * x.x;
+    o.y += f * x.y;
+    o.z += f * x.z;
+    o.w += f * x.w;
+  }
+  s_o[warp * kSide + sub][t] = o;
+  __syncthreads();
+  if (tid < kLanes) {
+    o = s_o[0][tid];
+#pragma unroll
+    for (int v = 1; v < kMergeWarps * kSide; ++v) {
+      const float4 x = s_o[v][tid];
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
+    }
+    const float inv = 1.f / l;
+    uint8_t* op = reinterpret_cast<uint8_t*>(a.out) + 2 * (static_cast<int64_t>(b) * a.out_stride[0] + static_cast<int64_t>(h) * a.out_stride[1]);
+    uint2 r = make_uint2(0u, 0u);
+    if (!no_result<true>(l)) r = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint2*>(op + 8 * tid) = r;
+  }
+}
+
+// set-once function attributes per device; the attribute calls themselves are idempotent
+template <class F>
+cudaError_t once_per_device(std::atomic<bool> (&done)[64], F&& set) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev >= 64 || !done[dev].load(std::memory_order_acquire)) {
+    e = set();
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
   }
+  return cudaSuccess;
+}
+
+template <int D, bool BF16, bool I8, bool Paged, int NT, int kSt>
+cudaError_t launch_ring(const DecodeB8Args& a, cudaStream_t stream) {
+  auto* kernel = decode_b8_kernel<D, BF16, I8, Paged, NT, kSt>;
+  constexpr int smem = LayoutB8<D, NT, kSt>::kBytes;
+  static std::atomic<bool> done[64] = {};
+  cudaError_t e = once_per_device(done, [&] {
+    const cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return x != cudaSuccess ? x : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (e != cudaSuccess) return e;
   const bool clustered = a.part_o == nullptr;
   LaunchAttrs at(stream);
   at.cfg.gridDim = dim3(a.n_split, a.n_kv_heads, a.batch);
@@ -411,8 +510,13 @@ cudaError_t launch_heads(const DecodeB8Args& a, cudaStream_t stream) {
   if (e != cudaSuccess || clustered) return e;
   LaunchAttrs ac(stream);
   ac.cfg.gridDim = dim3(a.n_heads, a.batch);
-  ac.cfg.blockDim = dim3(D);
-  return cudaLaunchKernelEx(&ac.cfg, decode_combine_kernel<D, BF16, true>, static_cast<const DecodeArgs&>(a));
+  ac.cfg.blockDim = dim3(32 * kMergeWarps);
+  return cudaLaunchKernelEx(&ac.cfg, decode_b8_merge_kernel<D, BF16>, a);
+}
+
+template <int D, bool BF16, bool I8, bool Paged, int NT>
+cudaError_t launch_heads(const DecodeB8Args& a, cudaStream_t stream) {
+  return a.deep ? launch_ring<D, BF16, I8, Paged, NT, kDeep>(a, stream) : launch_ring<D, BF16, I8, Paged, NT, kShallow>(a, stream);
 }
 
 template <int D, bool BF16, bool I8>

@@ -177,7 +177,7 @@ __device__ __forceinline__ void merge_partials(const DecodeArgs& a, uint8_t* sme
 
 // The merge is a latency problem (a few hundred bytes per thread, every load a trip to L2 or HBM), so the loads are
 // issued eight at a time: the (max, sum) pairs of eight splits, then the eight partial outputs they weight.
-template <int D, bool BF16, bool kKeepNan = false>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeArgs a) {
   const int h = blockIdx.x;
   const int b = blockIdx.y;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(D) decode_combine_kernel(const DecodeArgs a) {
       o += sc * x[j];
     }
   }
-  const float r = no_result<kKeepNan>(l) ? 0.f : o / l;
+  const float r = (l > 0.f) ? o / l : 0.f;
   uint8_t* op = reinterpret_cast<uint8_t*>(a.out) +
                 2 * (static_cast<size_t>(b) * a.out_stride[0] + static_cast<size_t>(h) * a.out_stride[1] + d);
   if constexpr (BF16) *reinterpret_cast<__nv_bfloat16*>(op) = __float2bfloat16_rn(r);
