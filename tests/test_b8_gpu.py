@@ -377,3 +377,79 @@ def test_prompt_chunk_and_tokens_together(kerns, fmt, page):
             dec(qt, *t, block, *table, lens, out)
             want, tol = O.b8_decode(qt.cpu(), c.values(0), c.values(1), lens.cpu(), torch.bfloat16)
             assert ((out.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt,dtype,B,H,Hkv,D,block,page,rows,lens", [
+    ("e4m3", torch.float16, 1, 32, 8, 128, 64, 0, 16400, [16400]), ("int8", torch.bfloat16, 3, 6, 1, 64, 16, 96, 87456, [87456, 0, 33]),
+    ("e4m3", torch.bfloat16, 1, 20, 2, 64, 128, 0, 131100, [131075]), ("int8", torch.float16, 2, 22, 2, 128, 32, 0, 33000, [17, 32999]),
+    ("e4m3", torch.float16, 24, 1, 1, 128, 128, 0, 5500, None)])
+def test_decode_split_over_all_sms(kerns, fmt, dtype, B, H, Hkv, D, block, page, rows, lens):
+    """Few pairs of a long padded cache: partial outputs through the workspace; long, short, empty and padded sequences alike."""
+    from minfer.kernels.torch_ext import _lib
+    assert _lib.lib.minfer_attn_decode_b8_workspace_bytes(B, H, Hkv, rows, D) > 0, "this shape is to take the split form"
+    c = Cache(fmt, B, Hkv, rows, D, block, page, seed=rows)
+    g = torch.Generator().manual_seed(B)
+    lens = torch.tensor(lens, dtype=torch.int32) if lens else torch.randint(0, rows + 1, (B,), generator=g, dtype=torch.int32)
+    check_decode(kerns, c, torch.randn(B, H, 1, D, generator=g).to(dtype), lens, dtype)
+
+
+def test_split_decode_in_two_graphs_and_on_two_streams(kerns):
+    """Calls that use a workspace at the same time: each has its own."""
+    D, H, Hkv, rows = 128, 8, 2, 66000
+    caches = [Cache("e4m3", 1, Hkv, rows, D, 128, seed=50 + i) for i in range(2)]
+    lens = torch.tensor([rows], dtype=torch.int32)
+    ts, ld = [c.to_gpu() for c in caches], lens.cuda()
+    qs = [torch.randn(1, H, 1, D, generator=torch.Generator().manual_seed(i)).half() for i in range(2)]
+    qd, outs = [q.cuda() for q in qs], [torch.zeros(1, H, 1, D, dtype=torch.float16, device="cuda") for _ in range(2)]
+    call = lambda i: kerns.flash_attn_decode_b8(qd[i], *ts[i], 128, ld, outs[i])  # noqa: E731
+    for i in range(2):
+        call(i)
+    torch.cuda.synchronize()
+    want = [o.clone() for o in outs]
+    for i, c in enumerate(caches):
+        ref, tol = O.b8_decode(qs[i], c.values(0), c.values(1), lens, torch.float16)
+        assert ((want[i].cpu().double() - ref).abs() <= tol).all()
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            call(i)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for run in (lambda i: graphs[i].replay(), call):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    run(i)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_codes_of_other_writers(kerns):
+    """Scales that are no power of two, the int8 code -128, negative zero and every finite e4m3 code: what another program wrote is read as
+    code * scale, and an append behind it codes the rows again from those values."""
+    D, block = 64, 16
+    for fmt in ("e4m3", "int8"):
+        c = Cache(fmt, 1, 1, 48, D, block, seed=6)
+        every = torch.arange(256, dtype=torch.uint8)
+        if fmt == "e4m3":
+            every = every[(every & 0x7F) != 0x7F]
+        vals = every.view(torch.float8_e4m3fn if fmt == "e4m3" else torch.int8).float().double()
+        for i in range(2):
+            c.codes[i][0, 0, :32] = vals.repeat(9)[:32 * D].view(32, D)
+            c.scale[i][0, 0] = torch.tensor([0.0123, 0.7, 1.9]).double()
+        check_decode(kerns, c, torch.randn(1, 2, 1, D, generator=torch.Generator().manual_seed(1)).half(), torch.tensor([32], dtype=torch.int32), torch.float16)
+        t = c.to_gpu()
+        ko, vo = (torch.zeros(1, 1, 32, D, dtype=torch.float16, device="cuda") for _ in range(2))
+        kerns.kv_read_b8(*t, block, torch.tensor([32], dtype=torch.int32, device="cuda"), ko, vo)
+        assert torch.equal(ko.cpu(), c.values(0)[:, :, :32].float().half()) and torch.equal(vo.cpu(), c.values(1)[:, :, :32].float().half())
+        for L in (1, 5):                                           # grows the block that holds rows 16 .. 26
+            t = c.to_gpu()
+            x = torch.full((1, L, 1, D), 3000.0, dtype=torch.float16)
+            append(kerns, c, t, 0, 0, x.cuda(), x.cuda(), x.cuda(), torch.tensor([27], dtype=torch.int32))
+            torch.cuda.synchronize()
+            got_c, got_s = c.back(t[0], t[2])
+            want_c, want_s = O.b8_append(c.codes[0][0, 0], c.scale[0][0, 0], x[0, :, 0].double(), 27, block, c.int8)
+            assert torch.equal(got_c[0, 0], want_c) and torch.equal(got_s[0, 0], want_s), (fmt, L)
