@@ -31,8 +31,11 @@ namespace {
 constexpr int kRowThreads = 128;    // a block that works on rows
 constexpr int kThreads = 256;       // a block that works on blocks of a cache (and, behind those, on rows)
 constexpr int kMaxPairs = 128;      // rotated pairs of a head
-constexpr int kStages = 3;  // steps of two rows per thread on their way through shared memory (no registers held while they fly)
-constexpr int rows_smem(int threads) { return kStages * 4 * threads * static_cast<int>(sizeof(uint4)); }
+// Rows per thread in a step of rows_role - two give two independent chains; the rows of an 8-bit cache need the registers for their codes -
+// and steps on their way through shared memory (no registers held while they fly).
+constexpr int rows_per_step(int fmt) { return fmt == 0 ? 2 : 1; }
+constexpr int ring_stages(int rows) { return rows == 1 ? 4 : 3; }
+constexpr int rows_smem(int threads, int rows) { return ring_stages(rows) * 2 * rows * threads * static_cast<int>(sizeof(uint4)); }
 
 template <bool BF16>
 __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
@@ -288,18 +291,19 @@ __device__ __forceinline__ bool locate(const NormRopeArgs& a, int b, int pos, bo
 // sequence, whose row alone decides about its block ----
 //
 // A warp takes a token (or, with few tokens, one of `slices` shares of its rows): nothing is shared between warps, no barrier.  Its
-// 32 / TPR row groups walk the query heads, the k heads and the v heads side by side, two rows each per step (two independent chains
+// 32 / TPR row groups walk the query heads, the k heads and the v heads side by side, kR rows each per step (two independent chains
 // of reduction and arithmetic).  A thread brings its own pieces of the next steps into shared memory with asynchronous copies.  The
 // token's angles stay in registers for all rows, the weights too unless every head has its own.
-struct Cursor {  // of one row group: its two rows of a step
+struct Cursor {  // of one row group: its rows of a step
   int s, row, n;
   int kind;            // 0 q, 1 k, 2 v
-  int64_t off, step;   // bytes from the kind's base: of the first row, between its two rows
+  int64_t off, step;   // bytes from the kind's base: of the first row, from row to row
 };
 
-template <int TPR, bool BF16, bool kNeox, int kFmt, int kT>
+template <int TPR, bool BF16, bool kNeox, int kFmt, int kT, int kR>
 __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, unsigned slices, int n_k, int n_v, const uint64_t* s_turns, uint4* s_rows) {
   constexpr int kSide = 32 / TPR;  // row groups of a warp
+  constexpr int kSt = ring_stages(kR);
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & 31;
   const int t = lane % TPR, group = lane / TPR;
@@ -309,8 +313,8 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   const int l = static_cast<int>(token - static_cast<unsigned>(b) * static_cast<unsigned>(a.seq));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int n_q = a.q != nullptr ? a.n_heads : 0;
-  // steps of 2 kSide rows: q's, k's, v's; this warp's are [s0, s1)
-  const int q_steps = (n_q + 2 * kSide - 1) / (2 * kSide), k_steps = (n_k + 2 * kSide - 1) / (2 * kSide), v_steps = (n_v + 2 * kSide - 1) / (2 * kSide);
+  // steps of kR kSide rows: q's, k's, v's; this warp's are [s0, s1)
+  const int q_steps = (n_q + kR * kSide - 1) / (kR * kSide), k_steps = (n_k + kR * kSide - 1) / (kR * kSide), v_steps = (n_v + kR * kSide - 1) / (kR * kSide);
   const int steps = q_steps + k_steps + v_steps;
   const int s0 = static_cast<int>(static_cast<unsigned>(steps) * slice / slices), s1 = static_cast<int>(static_cast<unsigned>(steps) * (slice + 1) / slices);
   uint8_t* q_base = reinterpret_cast<uint8_t*>(a.q) + 2 * (static_cast<int64_t>(b) * a.q_stride[0] + static_cast<int64_t>(l) * a.q_stride[1]);
@@ -320,7 +324,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
 
   auto enter = [&](Cursor& c) {  // the kind that step c.s belongs to
     c.kind = c.s < q_steps ? 0 : c.s < q_steps + k_steps ? 1 : 2;
-    c.row = (c.s - (c.kind == 0 ? 0 : c.kind == 1 ? q_steps : q_steps + k_steps)) * 2 * kSide + group;
+    c.row = (c.s - (c.kind == 0 ? 0 : c.kind == 1 ? q_steps : q_steps + k_steps)) * kR * kSide + group;
     c.n = c.kind == 0 ? n_q : c.kind == 1 ? n_k : n_v;
     const int64_t stride = 2 * (c.kind == 0 ? a.q_stride[2] : a.kv_stride[2]);
     c.off = c.row * stride;
@@ -328,8 +332,8 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   };
   auto advance = [&](Cursor& c) {
     ++c.s;
-    c.row += 2 * kSide;
-    c.off += 2 * c.step;
+    c.row += kR * kSide;
+    c.off += kR * c.step;
     if (c.s == q_steps || c.s == q_steps + k_steps) enter(c);
   };
   Cursor in;  // the step to be fetched next
@@ -338,9 +342,9 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   auto issue = [&](int stage) {
     if (in.s < s1) {
       const uint8_t* src = (in.kind == 0 ? q_base : in.kind == 1 ? k_base : v_base) + in.off;
-      uint4* dst = s_rows + stage * 4 * kT + tid;
+      uint4* dst = s_rows + stage * (2 * kR) * kT + tid;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < kR; ++u) {
         if (ch.live && in.row + u * kSide < in.n) {
           cp_async_16(dst + (2 * u) * kT, src + u * in.step + 16 * ch.c0, true);
           cp_async_16(dst + (2 * u + 1) * kT, src + u * in.step + 16 * ch.c1, true);
@@ -351,9 +355,9 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(i);  // on their way before the position is known
+  for (int i = 0; i < kSt - 1; ++i) issue(i);  // on their way before the position is known
 
-  const int pos = (a.start != nullptr ? a.start[b] : a.start_pos) + l;
+  const int pos = static_cast<int>(static_cast<unsigned>(a.start != nullptr ? a.start[b] : a.start_pos) + static_cast<unsigned>(l));
   int outer = 0, crow = 0;
   bool cache_ok = false;
   if (a.k_cache != nullptr && s1 > q_steps) cache_ok = locate(a, b, pos, lane == 0, outer, crow);
@@ -368,20 +372,20 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   enter(at);
   int stage = 0;
   for (; at.s < s1; advance(at)) {
-    cp_async_wait<kStages - 2>();
-    const uint4* sp = s_rows + stage * 4 * kT + tid;
-    const bool both = at.row - group + kSide < at.n;  // rows for the second half of the step
-    uint4 raw[2][2];
+    cp_async_wait<kSt - 2>();
+    const uint4* sp = s_rows + stage * (2 * kR) * kT + tid;
+    const bool both = kR == 2 && at.row - group + kSide < at.n;  // rows for the second half of the step
+    uint4 raw[kR][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kR; ++u) {
       const bool there = ch.live && at.row + u * kSide < at.n;
       raw[u][0] = there ? sp[(2 * u) * kT] : make_uint4(0, 0, 0, 0);
       raw[u][1] = there ? sp[(2 * u + 1) * kT] : make_uint4(0, 0, 0, 0);
     }
-    issue(stage == 0 ? kStages - 1 : stage - 1);
-    stage = stage == kStages - 1 ? 0 : stage + 1;
+    issue(stage == 0 ? kSt - 1 : stage - 1);
+    stage = stage == kSt - 1 ? 0 : stage + 1;
     const int kind = at.kind;
-    float x[2][16];
+    float x[kR][16];
     auto turn = [&](auto rows) {  // norm, weights and rotation of one row or two
       constexpr int kRows = decltype(rows)::value;
       const int64_t w_stride = (kind == 0 ? a.w_stride[0] : a.w_stride[1]) * w_bytes;
@@ -418,7 +422,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
       }
     };
     if (kind != 2) {
-      if (both) turn(std::integral_constant<int, 2>{});
+      if (both) turn(std::integral_constant<int, kR>{});
       else turn(std::integral_constant<int, 1>{});
     }
     if (kFmt == 0 || kind == 0) {
@@ -434,7 +438,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
         dst_step = 2 * kSide * a.cache_stride[1];
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < kR; ++u) {
         if (!ch.live || at.row + u * kSide >= at.n) continue;
         *reinterpret_cast<uint4*>(dst + u * dst_step + 16 * ch.c0) = raw[u][0];
         *reinterpret_cast<uint4*>(dst + u * dst_step + 16 * ch.c1) = raw[u][1];
@@ -443,34 +447,33 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
       if (!cache_ok) continue;
       const int begun = crow & ((1 << a.log_block) - 1);  // rows of the block that are there
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < kR; ++u) {
         if (u == 1 && !both) break;
+        const int h = at.row + u * kSide;
+        const bool row_ok = h < at.n;
+        float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
+        const float o0 = row_ok && begun != 0 ? *sc : 0.f;  // the block's scale before and after
         if (kind == 2) {
           unpack8<BF16>(raw[u][0], x[u]);
           unpack8<BF16>(raw[u][1], x[u] + 8);
         }
-        const int h = at.row + u * kSide;
-        const bool row_ok = h < at.n;
         float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[u][i]));
+        for (int i = 0; i < 8; ++i) amax = fmax3(amax, fabsf(x[u][2 * i]), fabsf(x[u][2 * i + 1]));
 #pragma unroll
         for (int d = TPR / 2; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, d));
-        uint8_t* blk_rows = nullptr;
-        float o0 = 0.f, o1 = 0.f;                           // the block's scale before and after
+        const float need = b8_scale<kFmt>(amax);
+        const float o1 = o0 >= need ? o0 : need;
+        uint8_t* blk_rows = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
+                            static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
         if (row_ok) {
-          float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
-          blk_rows = reinterpret_cast<uint8_t*>(kind == 1 ? a.k_cache : a.v_cache) + static_cast<int64_t>(outer) * a.cache_stride[0] +
-                     static_cast<int64_t>(h) * a.cache_stride[1] + static_cast<int64_t>(crow - begun) * a.cache_stride[2];
-          o0 = begun != 0 ? *sc : 0.f;
-          const float need = b8_scale<kFmt>(amax);
-          o1 = o0 >= need ? o0 : need;
           const float r1 = b8_inverse(o1);
           uint8_t* dst = blk_rows + static_cast<int64_t>(begun) * a.cache_stride[2];
           *reinterpret_cast<uint2*>(dst + 8 * ch.c0) = b8_code8<kFmt>(x[u], o1, r1);
           *reinterpret_cast<uint2*>(dst + 8 * ch.c1) = b8_code8<kFmt>(x[u] + 8, o1, r1);
-          if (t == 0 && (begun == 0 || o1 != o0)) *sc = o1;  // (a block that begins here held anything)
         }
+        __syncwarp();  // every lane of the row has read the scale
+        if (row_ok && t == 0 && (begun == 0 || o1 != o0)) *sc = o1;  // (a block that begins here held anything)
         // A scale that grew: the rows before are coded again, by the whole warp
         unsigned grown = __ballot_sync(0xFFFFFFFFu, row_ok && begun != 0 && o1 != o0 && t == 0);
         while (grown != 0) {
@@ -487,12 +490,13 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
 
 template <int TPR, bool BF16, bool kNeox, int kFmt>
 __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const NormRopeArgs a) {
-  __shared__ __align__(16) uint4 s_rows[rows_smem(kRowThreads) / sizeof(uint4)];
+  constexpr int kR = rows_per_step(kFmt);
+  __shared__ __align__(16) uint4 s_rows[rows_smem(kRowThreads, kR) / sizeof(uint4)];
   __shared__ uint64_t s_turns[kMaxPairs];
   grid_launch_dependents();
   copy_turns<kRowThreads>(a, s_turns);
   grid_dependency_wait();
-  rows_role<TPR, BF16, kNeox, kFmt, kRowThreads>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
+  rows_role<TPR, BF16, kNeox, kFmt, kRowThreads, kR>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
                                                  a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_turns, s_rows);
 }
 
@@ -704,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
     if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
     else block_role<TPR, BF16, kNeox, kFmt, true, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
   } else {
-    rows_role<TPR, BF16, kNeox, 0, kThreads>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
+    rows_role<TPR, BF16, kNeox, 0, kThreads, 2>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
                                              s_turns, reinterpret_cast<uint4*>(s_dyn));
   }
 }
@@ -776,7 +780,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   const int fmt = cache_format == MINFER_ATTN_KV_E4M3 ? kE4M3 : cache_format == MINFER_ATTN_KV_INT8 ? kInt8 : 0;
   const bool by_block = fmt != 0 && a.seq > 1;
   const int kv_rows = by_block ? 0 : a.n_kv_heads;
-  const int step_rows = 2 * side;
+  const int step_rows = (by_block ? 2 : rows_per_step(fmt)) * side;
   const int steps = (a.q != nullptr ? (a.n_heads + step_rows - 1) / step_rows : 0) + (a.k != nullptr ? (kv_rows + step_rows - 1) / step_rows : 0) +
                     (a.v != nullptr ? (kv_rows + step_rows - 1) / step_rows : 0);
   // A warp takes a token; while that leaves the GPU's warps (16 per SM) without work, a token's rows are dealt out over several.
@@ -813,7 +817,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   const long long blocks = 2 * units * kv_slices + (a.q != nullptr ? row_blocks : 0);
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
   size_t smem = blocks_smem((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads, true);
-  if (a.q != nullptr && smem < static_cast<size_t>(rows_smem(kThreads))) smem = rows_smem(kThreads);
+  if (a.q != nullptr && smem < static_cast<size_t>(rows_smem(kThreads, 2))) smem = rows_smem(kThreads, 2);
   const unsigned nb = static_cast<unsigned>(blocks);
   if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kE4M3, a, nb, smem, stream);
   return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kInt8, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kInt8, a, nb, smem, stream);
