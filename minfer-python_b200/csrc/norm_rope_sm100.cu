@@ -88,12 +88,16 @@ struct Chunks {
 };
 
 // cos and sin of pair i at a position.  The table is read from shared memory: in the kernel's arguments, lanes that want
-// different entries would be served one after another.
+// different entries would be served one after another.  The nearest quarter turn is split off in integers, so that what is rounded to fp32 is an
+// eighth of a turn at most: a whole half turn would be rounded by up to pi 2^-25, several times what cos and sin themselves are.
 __device__ __forceinline__ float2 angle_of(const uint64_t* s_turns, int pos, int i) {
   const uint64_t turns = static_cast<uint64_t>(static_cast<int64_t>(pos)) * s_turns[i];
+  const uint32_t hi = static_cast<uint32_t>(turns >> 32);
+  const uint32_t quarters = (hi + 0x20000000u) >> 30;
   float s, c;
-  sincospif(static_cast<float>(static_cast<int32_t>(turns >> 32)) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31: half turns
-  return make_float2(c, s);
+  sincospif(static_cast<float>(static_cast<int32_t>(hi - (quarters << 30))) * 4.656612873077392578125e-10f, &s, &c);  // 2^-31: half turns
+  const float x = (quarters & 1u) ? s : c, y = (quarters & 1u) ? c : s;
+  return make_float2(((quarters + 1u) & 2u) ? -x : x, (quarters & 2u) ? -y : y);
 }
 
 template <int kT>
@@ -506,9 +510,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const No
 // lanes: four, two or one head at a time, or two or four rows per thread.  The raw rows come through shared memory, each thread's own
 // pieces (no barrier; the next head's are fetched as soon as these have been read); k's normed and rotated rows wait there in
 // fp32 until the block's largest magnitude is agreed on.  A thread computes the angles of its first row once for all heads of the
-// unit and turns them on from row to row by the angle between two of its rows (three times at most, an error of 2^-24 each).
-constexpr int blocks_smem(int lanes, bool k) {  // lanes that the rows of the heads side by side fill (kThreads at least)
-  return 2 * kMaxPairs * 4 + lanes * 32 + (k ? lanes * 64 : 0);
+// unit and turns those on to each of its other rows, by the angle between the two: one product, whatever the row (from row to row
+// its roundings would add up, and more values fall on the wrong side of a border between two codes).
+constexpr int kMaxRows = 4;                          // of a thread
+constexpr int kTurnFloats = (kMaxRows - 1) * 2 * kMaxPairs;  // cos and sin of the angles to rows 1, 2, 3
+constexpr int blocks_smem(int lanes) {  // lanes that the rows of the heads side by side fill (kThreads at least)
+  return kTurnFloats * 4 + lanes * (32 + 64);
 }
 
 // largest magnitude of a row's raw values (NaN is passed over)
@@ -535,10 +542,9 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   const int blk = 1 << a.log_block;
   const int pairs = a.rotary_dim / 2;
   const int side = max(1, kThreads / (blk * TPR));               // heads side by side
-  float* s_cos = smem;                                           // of the angle between two rows of a thread
-  float* s_sin = smem + kMaxPairs;
-  uint4* s_raw = reinterpret_cast<uint4*>(smem + 2 * kMaxPairs) + tid;                    // [kRows][2] pieces, kThreads apart
-  float4* s_val = reinterpret_cast<float4*>(smem + 2 * kMaxPairs) + kRows * 2 * kThreads + tid;  // [kRows][4]: k as it is to be coded
+  float* s_turn = smem;                                          // [kMaxRows - 1][2][kMaxPairs]
+  uint4* s_raw = reinterpret_cast<uint4*>(smem + kTurnFloats) + tid;                    // [kRows][2] pieces, kThreads apart
+  float4* s_val = reinterpret_cast<float4*>(smem + kTurnFloats) + kRows * 2 * kThreads + tid;  // [kRows][4]: k as it is to be coded
   const int b = static_cast<int>(unit / static_cast<unsigned>(a.n_touch)), j = static_cast<int>(unit - static_cast<unsigned>(b) * static_cast<unsigned>(a.n_touch));
   const Chunks<kNeox> ch(t, a.head_dim, a.rotary_dim);
   const int64_t start = a.start != nullptr ? a.start[b] : a.start_pos;
@@ -579,10 +585,12 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
   Angles first = {};
   if (kIsK && pairs > 0) {
     if (kRows > 1) {
-      for (int u = tid; u < pairs; u += kThreads) {
-        const float2 cs = angle_of(s_turns, row_step, u);
-        s_cos[u] = cs.x;
-        s_sin[u] = cs.y;
+      for (int u = tid; u < (kRows - 1) * kMaxPairs; u += kThreads) {
+        const int r = u / kMaxPairs, i = u % kMaxPairs;
+        if (i >= pairs) continue;
+        const float2 cs = angle_of(s_turns, (r + 1) * row_step, i);
+        s_turn[2 * r * kMaxPairs + i] = cs.x;
+        s_turn[(2 * r + 1) * kMaxPairs + i] = cs.y;
       }
       __syncthreads();
     }
@@ -622,14 +630,14 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
         amax = fmaxf(amax, raw_amax<BF16>(raw0, raw1));
       } else {
         fetch(g + 1, r);
-        if (r > 0) {  // the angles of the thread's next row
+        if (r > 0) {  // the angles of the thread's r-th row
           Angles d = {};
-          load_angles<kNeox>(s_cos, s_sin, ch, d);
+          load_angles<kNeox>(s_turn + 2 * (r - 1) * kMaxPairs, s_turn + (2 * r - 1) * kMaxPairs, ch, d);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 c = angles.c[i];
-            angles.c[i] = __ffma2_rn(angles.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
-            angles.s[i] = __ffma2_rn(angles.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
+            const float2 c = first.c[i];
+            angles.c[i] = __ffma2_rn(first.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
+            angles.s[i] = __ffma2_rn(first.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
             angles.n[i] = make_float2(-angles.s[i].x, -angles.s[i].y);
           }
         }
@@ -816,7 +824,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   a.kv_slices = static_cast<int>(kv_slices);
   const long long blocks = 2 * units * kv_slices + (a.q != nullptr ? row_blocks : 0);
   if (blocks > 0x7FFFFFFFll) return cudaErrorInvalidValue;
-  size_t smem = blocks_smem((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads, true);
+  size_t smem = blocks_smem((tpr << a.log_block) > kThreads ? tpr << a.log_block : kThreads);
   if (a.q != nullptr && smem < static_cast<size_t>(rows_smem(kThreads, 2))) smem = rows_smem(kThreads, 2);
   const unsigned nb = static_cast<unsigned>(blocks);
   if (fmt == kE4M3) return tpr == 4 ? MINFER_NR_STYLE(launch_blocks, 4, kE4M3, a, nb, smem, stream) : MINFER_NR_STYLE(launch_blocks, 8, kE4M3, a, nb, smem, stream);

@@ -453,3 +453,30 @@ def test_codes_of_other_writers(kerns):
             got_c, got_s = c.back(t[0], t[2])
             want_c, want_s = O.b8_append(c.codes[0][0, 0], c.scale[0][0, 0], x[0, :, 0].double(), 27, block, c.int8)
             assert torch.equal(got_c[0, 0], want_c) and torch.equal(got_s[0, 0], want_s), (fmt, L)
+
+
+@pytest.mark.parametrize("block", [16, 64, 128])
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("start", [0, 100_000])
+def test_angles_are_exact_to_fp32(kerns, block, style, start):
+    """An int8 block with one value in it has that value's magnitude / 127 as its scale, in 32 bits: with 1 in one half of a pair, the
+    larger of |cos| and |sin| of that pair's angle."""
+    d, n = 64, 8 * block
+    first = start // block * block
+    k = torch.zeros(1, n, 1, d, dtype=torch.float16, device="cuda")
+    rows = torch.arange(8) * block + (torch.arange(8) * 37 + 5) % block
+    pair = torch.arange(8) * 5 % (d // 2)
+    k[0, rows, 0, pair * 2 if style == 0 else pair] = 1.0
+    q = torch.zeros(1, n, 1, d, dtype=torch.float16, device="cuda")
+    lmax = first + n
+    kc, vc = (torch.zeros(1, 1, lmax, d, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(1, 1, (lmax + block - 1) // block, device="cuda") for _ in range(2))
+    kerns.rope_kv_append_b8(d, 10000.0, style, q, k, torch.zeros_like(k), kc, vc, ks, vs, block,
+                            torch.tensor([first], dtype=torch.int32, device="cuda"))
+    got = ks[0, 0, first // block:].double().cpu() * 127
+    angle = (first + rows).double() * 10000.0 ** (-2.0 * pair.double() / d)
+    want = torch.maximum(angle.cos().abs(), angle.sin().abs())
+    # In units of 2^-24: sincospif is within 1 of values below 1, its argument (an eighth of a turn) is rounded by pi / 8; a row's angle
+    # is the sum of two such, (1 + pi / 8) * 2 * sqrt 2 = 3.94, and the sum's two roundings make it 4.94; relative to sqrt 1/2 or more 6.99,
+    # and the scale's own rounding is 1.
+    assert ((got - want).abs() / want).max() <= 8 * 2.0 ** -24
