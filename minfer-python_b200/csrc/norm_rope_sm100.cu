@@ -14,6 +14,10 @@
 //
 // A row (one head of one token) belongs to TPR = 4, 8 or 16 lanes with two 16-byte chunks each; in the two-halves form they are a chunk and
 // its partner, so a rotated pair never leaves its thread.
+//
+// Measured (32 / 8 heads, D=128, 4 x 4096 tokens, back to back): 16-bit cache 63.9 us, 6.3 TB/s, 0.98 of what a copy reaches; 8-bit cache (e4m3,
+// blocks of 128) 76.4 us, 4.8 TB/s, bound by issue slots (55 % busy) and latency at 16 warps per SM; single tokens of 64 sequences 3.0 and
+// 3.1 us, launch and latency.
 #include "../../include/minfer_attn.h"
 #include "attn_internal.h"
 #include "b8.cuh"
