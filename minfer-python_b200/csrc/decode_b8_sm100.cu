@@ -330,10 +330,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kSt == kShallow ? 3 : 
     len = max(0, min(a.lens[b], a.max_len));
   }
   // the keys of this block: an even share of the sequence's tiles
-  const int nt_seq = (len + kTileKeys - 1) / kTileKeys;
-  const int c0 = static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part) / static_cast<unsigned>(n_parts)) * kTileKeys;
-  const int c1 = min(len, static_cast<int>(static_cast<unsigned>(nt_seq) * static_cast<unsigned>(part + 1) / static_cast<unsigned>(n_parts)) * kTileKeys);
-  const int nt = c1 > c0 ? (c1 - c0 + kTileKeys - 1) / kTileKeys : 0;
+  // (quotient and remainder: the product of the tiles and a block's number passes 32 bits from 231 million keys on)
+  const unsigned nt_seq = (static_cast<unsigned>(len) + kTileKeys - 1) / kTileKeys;
+  const unsigned share = nt_seq / static_cast<unsigned>(n_parts), more = nt_seq - share * static_cast<unsigned>(n_parts);  // `more` blocks take one more
+  const unsigned t0 = share * static_cast<unsigned>(part) + min(static_cast<unsigned>(part), more);
+  const int c0 = static_cast<int>(min(static_cast<unsigned>(len), t0 * kTileKeys));
+  const int c1 = static_cast<int>(min(static_cast<unsigned>(len), (t0 + share + (static_cast<unsigned>(part) < more ? 1u : 0u)) * kTileKeys));
+  const int nt = (c1 - c0) / kTileKeys + ((c1 - c0) % kTileKeys != 0 ? 1 : 0);
   const int nt_w = (nt > warp) ? (nt - warp + kWarps - 1) / kWarps : 0;
 
   uint8_t* wsm = smem + warp * kWarpBytes;

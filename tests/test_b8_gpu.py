@@ -480,3 +480,21 @@ def test_angles_are_exact_to_fp32(kerns, block, style, start):
     # is the sum of two such, (1 + pi / 8) * 2 * sqrt 2 = 3.94, and the sum's two roundings make it 4.94; relative to sqrt 1/2 or more 6.99,
     # and the scale's own rounding is 1.
     assert ((got - want).abs() / want).max() <= 8 * 2.0 ** -24
+
+
+def test_decode_shares_of_a_sequence_that_pass_32_bits(kerns):
+    """301 million keys, nearly all of them the same page: keys of zeros weigh the same, so the output is the share of each page's values.
+    The last fifth of the table names the second page: shares that went wrong leave it out."""
+    page, n0, n1, d, block = 65536, 3700, 900, 64, 128
+    kc = torch.zeros(2, 1, page, d, device="cuda").to(torch.float8_e4m3fn)
+    vc = torch.ones(2, 1, page, d, device="cuda")
+    vc[1] = -1.0
+    s = torch.ones(2, 1, page // block, device="cuda")
+    table = torch.tensor([[0] * n0 + [1] * n1], dtype=torch.int32, device="cuda")
+    q = torch.ones(1, 1, 1, d, dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    kerns.flash_attn_decode_b8_paged(q, kc, vc.to(torch.float8_e4m3fn), s, s.clone(), block, table, torch.tensor([page * (n0 + n1)], dtype=torch.int32, device="cuda"), out)
+    want = (n0 - n1) / (n0 + n1)
+    # A warp's sums are of equal powers of two, fewer than 2^24: exact.  Adding up 296 blocks' (of 4 warps) parts rounds 300 times at most,
+    # in numerator and denominator; then one rounding to fp16.
+    assert (out.double() - want).abs().max() <= want * (2.0 ** -11 + 2 * 300 * 2.0 ** -24)
