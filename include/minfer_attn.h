@@ -355,6 +355,8 @@ int minfer_attn_rope_append(const MinferRopeParams* params, void* stream);
  *     start[b] are coded again from the values that they stood for.  It never shrinks.  Rows behind the last new one are not touched.
  * Positions outside [0, max_len) are not written (q is still rewritten) and reported through `status`, as are entries of the
  * block table outside [0, n_pages).  The caller sees to it that no two sequences append to the same page.
+ * What is written has a stride in every dimension of more than one entry; q is neither k nor v, k_cache (k_scale) not v_cache (v_scale).
+ * Without caches start[b] + seq has to stay below 2^31.
  */
 typedef struct MinferNormRopeParams {
   void*          q;
@@ -442,6 +444,7 @@ size_t minfer_attn_decode_b8_workspace_bytes(int32_t batch, int32_t n_heads, int
  * Rows of a b8 cache as 16-bit values (code * scale, rounded once): row j of sequence b to row j of k_out / v_out
  * [batch, n_kv_heads, out_rows, head_dim] for j < min(lens[b], max_len, out_rows); the other rows of the outputs are not touched.  For the
  * attention of a prompt behind a cached prefix (minfer_attn_prefill reads 16-bit keys and values).
+ * k_out and v_out are two buffers; min(max_len, out_rows) is at most 2^31 - 129.
  */
 typedef struct MinferKvReadB8Params {
   const void*    k_cache;

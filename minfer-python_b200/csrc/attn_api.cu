@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <cstring>
 #include <mutex>
 
@@ -200,6 +201,15 @@ bool b8_strides_ok(const int64_t cache[3], const int64_t scale[2]) {
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// What is written wants a stride in every dimension of more than one entry: several threads would rewrite the entries of an expanded tensor at once
+bool written_apart(const int64_t* stride, std::initializer_list<int64_t> extents) {
+  for (const int64_t n : extents) {
+    if (n > 1 && *stride == 0) return false;
+    ++stride;
+  }
+  return true;
+}
 
 // block_size > 0: pages have to hold whole blocks
 bool table_ok(const int32_t* table, int32_t page_size, int32_t table_stride, int32_t n_pages, int32_t max_len, int32_t block_size) {
@@ -595,6 +605,15 @@ int minfer_attn_norm_rope_append(const MinferNormRopeParams* p, void* stream) {
   if (p->start != nullptr && !aligned4(p->start)) return MINFER_ATTN_EINVAL;
   if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
   if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
+  // what is written is written once, and read by nobody else
+  if (p->q != nullptr && (p->q == p->k || (p->k_cache != nullptr && p->q == p->v) || !written_apart(p->q_stride, {p->batch, p->seq, p->n_heads}))) return MINFER_ATTN_EINVAL;
+  if (p->k_cache == nullptr) {
+    if (p->k != nullptr && !written_apart(p->kv_stride, {p->batch, p->seq, p->n_kv_heads})) return MINFER_ATTN_EINVAL;
+  } else {
+    const int64_t outer = p->block_table != nullptr ? p->n_pages : p->batch, rows = p->block_table != nullptr ? p->page_size : p->max_len;
+    if (p->k_cache == p->v_cache || !written_apart(p->cache_stride, {outer, p->n_kv_heads, rows})) return MINFER_ATTN_EINVAL;
+    if (b8 && (p->k_scale == p->v_scale || !written_apart(p->scale_stride, {outer, p->n_kv_heads}))) return MINFER_ATTN_EINVAL;
+  }
   int rc = check_device();
   if (rc != MINFER_ATTN_OK) return rc;
   NormRopeArgs a{};
@@ -663,6 +682,7 @@ int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* p, void* stream) {
   if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
   const size_t need = minfer_attn_decode_b8_workspace_bytes(p->batch, p->n_heads, p->n_kv_heads, p->max_len, p->head_dim);
   if (p->workspace != nullptr && need > 0 && (p->workspace_bytes < need || !aligned16(p->workspace))) return MINFER_ATTN_EWORKSPACE;
+  if (!written_apart(p->out_stride, {p->batch, p->n_heads})) return MINFER_ATTN_EINVAL;
   int rc = check_device();
   if (rc != MINFER_ATTN_OK) return rc;
 
@@ -723,6 +743,9 @@ int minfer_attn_kv_read_b8(const MinferKvReadB8Params* p, void* stream) {
   if (!table_ok(p->block_table, p->page_size, p->table_stride, p->n_pages, p->max_len, p->block_size)) return MINFER_ATTN_EINVAL;
   if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
   if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
+  const int64_t rows = std::min(p->max_len, p->out_rows);
+  if (rows > 0x7FFFFFFF - 128) return MINFER_ATTN_EINVAL;  // (rounded up to 128 in 32 bits)
+  if (p->k_out == p->v_out || !written_apart(p->out_stride, {p->batch, p->n_kv_heads, rows})) return MINFER_ATTN_EINVAL;
   int rc = check_device();
   if (rc != MINFER_ATTN_OK) return rc;
   KvReadArgs a{};

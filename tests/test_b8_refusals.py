@@ -138,3 +138,50 @@ def test_no_cpu_path():
                  lambda: k.kv_read_b8(c, c, s, s, 16, n, out16, out16.clone())):
         with pytest.raises(NotImplementedError):
             call()
+
+
+# These calls are right but for one argument, or altogether, and their addresses are made up: they must never meet a device.
+no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where no kernel can start")
+
+STRIDES = dict(q=0x10000, k=0x20000, v=0x30000, q_stride=(4096, 1024, 128), kv_stride=(768, 256, 128))
+CACHES = dict(k_cache=0x40000, v_cache=0x50000, cache_stride=(2 * 64 * 128, 64 * 128, 128))
+CACHES_B8 = dict(CACHES, k_scale=0x60000, v_scale=0x61000, scale_stride=(2, 1), cache_format=2, block_size=64)
+PAGES_B8 = dict(CACHES_B8, block_table=0x70000, page_size=64, table_stride=1, n_pages=3)
+
+
+@no_device
+@pytest.mark.parametrize("base,bad", [
+    ({}, dict(k=0x10000)), ({}, dict(q_stride=(0, 1024, 128))), ({}, dict(q_stride=(4096, 0, 128))), ({}, dict(q_stride=(4096, 1024, 0))),
+    ({}, dict(kv_stride=(0, 256, 128))), ({}, dict(kv_stride=(768, 0, 128))), ({}, dict(kv_stride=(768, 256, 0))),
+    (CACHES, dict(k=0x10000)), (CACHES, dict(v=0x10000)), (CACHES, dict(v_cache=0x40000)), (CACHES, dict(q_stride=(0, 1024, 128))),
+    (CACHES, dict(cache_stride=(0, 64 * 128, 128))), (CACHES, dict(cache_stride=(2 * 64 * 128, 0, 128))), (CACHES, dict(cache_stride=(2 * 64 * 128, 64 * 128, 0))),
+    (CACHES_B8, dict(v_cache=0x40000)), (CACHES_B8, dict(v_scale=0x60000)), (CACHES_B8, dict(scale_stride=(0, 1))), (CACHES_B8, dict(scale_stride=(2, 0))),
+    (PAGES_B8, dict(cache_stride=(0, 64 * 128, 128))), (PAGES_B8, dict(scale_stride=(0, 1)))])
+def test_what_is_written_lies_apart(lib, base, bad):
+    """Expanded tensors that are written, and one tensor given twice, are refused; the same call without them gets as far as the device."""
+    assert norm(lib, **STRIDES, **base) not in (EINVAL, EUNSUPPORTED)
+    assert norm(lib, **{**STRIDES, **base, **bad}) == EINVAL
+
+
+@no_device
+def test_expanded_inputs_are_read(lib):
+    """k and v that are only read, and dimensions of one entry, may have any stride."""
+    assert norm(lib, **{**STRIDES, **CACHES, "kv_stride": (0, 0, 0)}) not in (EINVAL, EUNSUPPORTED)
+    one = dict(batch=1, seq=1, n_heads=1, n_kv_heads=1, q_stride=(0, 0, 0), kv_stride=(0, 0, 0), cache_stride=(0, 0, 128))
+    assert norm(lib, **{**STRIDES, **CACHES, **one}) not in (EINVAL, EUNSUPPORTED)
+
+
+@no_device
+def test_outputs_lie_apart(lib):
+    dec = dict(q_stride=(1024, 128), out_stride=(1024, 128), out=0x20000)
+    call = lambda **kw: lib.lib.minfer_attn_decode_b8(ctypes.byref(fill(lib.DecodeB8Params(), DEC, {**dec, **kw})), None)  # noqa: E731
+    assert call() not in (EINVAL, EUNSUPPORTED)
+    assert call(out_stride=(0, 128)) == EINVAL and call(out_stride=(1024, 0)) == EINVAL and call(q_stride=(0, 0)) not in (EINVAL, EUNSUPPORTED)
+    read = dict(k_out=0x20000, v_out=0x30000, out_stride=(2 * 50 * 64, 50 * 64, 64))
+    call = lambda **kw: lib.lib.minfer_attn_kv_read_b8(ctypes.byref(fill(lib.KvReadB8Params(), READ, {**read, **kw})), None)  # noqa: E731
+    assert call() not in (EINVAL, EUNSUPPORTED)
+    assert call(v_out=0x20000) == EINVAL
+    for i in range(3):
+        assert call(out_stride=tuple(0 if j == i else x for j, x in enumerate(read["out_stride"]))) == EINVAL
+    assert call(batch=1, n_kv_heads=1, max_len=0x7FFFFFFF, out_rows=0x7FFFFFFF) == EINVAL      # row numbers are rounded up in 32 bits
+    assert call(batch=1, n_kv_heads=1, max_len=0x7FFFFFFF) not in (EINVAL, EUNSUPPORTED)        # the outputs have few
