@@ -738,13 +738,13 @@ int minfer_attn_kv_read_b8(const MinferKvReadB8Params* p, void* stream) {
   if (!aligned16(p->k_cache) || !aligned16(p->v_cache) || !aligned16(p->k_out) || !aligned16(p->v_out)) return MINFER_ATTN_EINVAL;
   if (!aligned4(p->k_scale) || !aligned4(p->v_scale) || !aligned4(p->lens)) return MINFER_ATTN_EINVAL;
   if (!strides_ok(p->out_stride, 3) || !b8_strides_ok(p->cache_stride, p->scale_stride)) return MINFER_ATTN_EINVAL;
-  // (sequence, head, 128 rows) triples are indexed in 32 bits
-  if ((static_cast<int64_t>(std::min(p->max_len, p->out_rows)) / 128 + 1) * p->batch * p->n_kv_heads >= (1ll << 31)) return MINFER_ATTN_EINVAL;
+  // (sequence, head, 32 rows) triples are indexed in 32 bits
+  if ((static_cast<int64_t>(std::min(p->max_len, p->out_rows)) / 32 + 1) * p->batch * p->n_kv_heads >= (1ll << 31)) return MINFER_ATTN_EINVAL;
   if (!table_ok(p->block_table, p->page_size, p->table_stride, p->n_pages, p->max_len, p->block_size)) return MINFER_ATTN_EINVAL;
   if (p->flags != 0) return MINFER_ATTN_EUNSUPPORTED;
   if (p->status != nullptr && !aligned4(p->status)) return MINFER_ATTN_EINVAL;
   const int64_t rows = std::min(p->max_len, p->out_rows);
-  if (rows > 0x7FFFFFFF - 128) return MINFER_ATTN_EINVAL;  // (rounded up to 128 in 32 bits)
+  if (rows > 0x7FFFFFFF - 128) return MINFER_ATTN_EINVAL;  // (rounded up to whole blocks in 32 bits)
   if (p->k_out == p->v_out || !written_apart(p->out_stride, {p->batch, p->n_kv_heads, rows})) return MINFER_ATTN_EINVAL;
   int rc = check_device();
   if (rc != MINFER_ATTN_OK) return rc;
