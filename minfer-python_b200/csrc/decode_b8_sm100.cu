@@ -23,7 +23,7 @@
 // 16-byte reads - K: chunks 2 tq and 2 tq + 1 of key g0; V: chunk g0 of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 - meet no bank twice.
 // A lane takes consecutive dimensions: for K that permutes the summands of an MMA, for V the rows of the output.
 //
-// Measured (32 / 8 heads, D=128, back to back): 64 sequences of 512-8192 keys, e4m3, 91.6 us, 6.2 TB/s, 0.97 of what a copy reaches; ragged
+// Measured (32 / 8 heads, D=128, back to back): 64 sequences of 512-8192 keys, e4m3, 91.9 us, 6.2 TB/s, 0.96 of what a copy reaches; ragged
 // int8 pages of 64 keys, 24 sequences of up to 10001 with 48 heads, 59.9 us, 0.68 (the same in one piece 52.8).
 #include "b8.cuh"
 #include "decode_common.cuh"
