@@ -498,3 +498,57 @@ def test_decode_shares_of_a_sequence_that_pass_32_bits(kerns):
     # A warp's sums are of equal powers of two, fewer than 2^24: exact.  Adding up 296 blocks' (of 4 warps) parts rounds 300 times at most,
     # in numerator and denominator; then one rounding to fp16.
     assert (out.double() - want).abs().max() <= want * (2.0 ** -11 + 2 * 300 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "16"])
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("seq", [1, 150])
+def test_offsets_that_pass_32_bits(kerns, fmt, paged, seq):
+    """The last sequence (the last page) of a cache lies beyond 2^32 bytes: append, read-back and decode give the same bits as in a small one."""
+    page, D, block = 1024, 64, 64
+    size = 2 if fmt == "16" else 1
+    far = (1 << 32) // (page * D * size) + 3                          # pages before the far one
+    dt = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8, "16": torch.float16}[fmt]
+    g = torch.Generator(device="cuda").manual_seed(seq)
+    q = torch.randn(2, seq, 4, D, generator=g, device="cuda", dtype=torch.float16)
+    k, v = (torch.randn(2, seq, 1, D, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    w = torch.rand(D, generator=g, device="cuda") + 0.5
+    start = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def run(last):
+        def laid(*shape, dtype):  # sequences (pages) 0 and `last`, with nothing else touched in between
+            step = shape[1] * shape[2] * (shape[3] if len(shape) == 4 else 1)
+            flat = torch.empty((last + 1) * step, dtype=dtype, device="cuda")
+            if paged:
+                t = flat.view(last + 1, *shape[1:])
+                ends = t.view(torch.int8) if dtype.itemsize == 1 else t
+            else:
+                strides = (last * step, step, *((shape[3], 1) if len(shape) == 4 else (1,)))
+                t = flat.as_strided(shape, strides)
+                ends = flat.view(torch.int8).as_strided(shape, strides) if dtype.itemsize == 1 else t
+            ends[0].zero_()
+            ends[-1].zero_()
+            return t
+        kc, vc = (laid(2, 1, page, D, dtype=dt) for _ in range(2))
+        table = torch.tensor([[0], [last]], dtype=torch.int32, device="cuda")
+        turn = (D, 10000.0, 0)
+        qq = q.clone()
+        pages = (table,) if paged else ()
+        if fmt == "16":
+            name = "qk_norm_rope_kv_append" + ("_paged" if paged else "")
+            getattr(kerns, name)(*turn, 1e-6, qq, k, v, w, w, kc, vc, *pages, start)
+            return [qq.cpu(), kc[0].cpu(), kc[-1].cpu(), vc[0].cpu(), vc[-1].cpu()]
+        ks, vs = (laid(2, 1, page // block, dtype=torch.float32) for _ in range(2))
+        tail = "_paged" if paged else ""
+        getattr(kerns, "rope_kv_append_b8" + tail)(*turn, qq, k, v, kc, vc, ks, vs, block, *pages, start, w, w, 1e-6)
+        lens = start + seq
+        ko, vo = (torch.zeros(2, 1, seq, D, dtype=torch.float16, device="cuda") for _ in range(2))
+        getattr(kerns, "kv_read_b8" + tail)(kc, vc, ks, vs, block, *pages, lens, ko, vo)
+        q1 = qq[:, -1:].transpose(1, 2).contiguous()
+        out = torch.empty_like(q1)
+        getattr(kerns, "flash_attn_decode_b8" + tail)(q1, kc, vc, ks, vs, block, *pages, lens, out)
+        return [qq.cpu(), *(raw(c[i].contiguous()).cpu() for c in (kc, vc) for i in (0, -1)), *(s[i].cpu() for s in (ks, vs) for i in (0, -1)), ko.cpu(), vo.cpu(), out.cpu()]
+
+    near, there = run(1), run(far)
+    assert all(torch.equal(a, b) for a, b in zip(near, there))
+    assert near[2].any() and near[4].any()                             # (something was written there)
