@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_b8_kernel(const KvReadArgs a
   const unsigned pair = blockIdx.x / per;   // sequence and head
   const int row0 = static_cast<int>(blockIdx.x - pair * per) * kRows + static_cast<int>(threadIdx.x) / 32 * 16;  // of this warp
   const int b = static_cast<int>(pair / static_cast<unsigned>(a.n_kv_heads)), h = static_cast<int>(pair - static_cast<unsigned>(b) * static_cast<unsigned>(a.n_kv_heads));
-  const int live = min(a.lens[b], a.max_len) - row0;  // rows of the 16 that there are
+  const int live = max(0, min(a.lens[b], a.max_len)) - row0;  // rows of the 16 that there are (a length near -2^31 less row0 would wrap to a huge one)
   if (live <= 0) return;
   const bool is_v = blockIdx.y != 0;
   int outer = b, r = row0;
