@@ -189,8 +189,14 @@ __device__ __forceinline__ void scale_pairs(Pairs& x, float f) {
 
 // A lane's angles; pairs that are not rotated are left out by apply_angles, not turned by 0 (an infinite value stays in its place).
 struct Angles {
-  float2 c[4], s[4], n[4];  // cos, sin, -sin
+  float2 c[4], s[4];  // cos, sin
 };
+
+// t - x * y: two scalar fmas, which negate for nothing.  Negated sines in registers and one packed fma instead made most of these kernels spill (norms, 4 x 4096 tokens,
+// bfloat16, two halves: 16-bit cache 72.9 us, now 64.6).
+__device__ __forceinline__ float2 minus_product(const float2& x, const float2& y, const float2& t) {
+  return make_float2(fmaf(-x.x, y.x, t.x), fmaf(-x.y, y.y, t.y));
+}
 
 template <bool kNeox>
 __device__ __forceinline__ void apply_angles(Pairs& x, const Angles& g, const Chunks<kNeox>& ch) {
@@ -198,7 +204,7 @@ __device__ __forceinline__ void apply_angles(Pairs& x, const Angles& g, const Ch
   for (int i = 0; i < 4; ++i) {
     if ((!kNeox && i >= 2) ? ch.rot1 : ch.rot0) {
       const float2 lo = x.lo[i], hi = x.hi[i];
-      x.lo[i] = __ffma2_rn(hi, g.n[i], __fmul2_rn(lo, g.c[i]));
+      x.lo[i] = minus_product(hi, g.s[i], __fmul2_rn(lo, g.c[i]));
       x.hi[i] = __ffma2_rn(lo, g.s[i], __fmul2_rn(hi, g.c[i]));
     }
   }
@@ -232,8 +238,6 @@ __device__ __forceinline__ void load_angles(const float* cosines, const float* s
       g.c[2 * h + 1] = make_float2(c.z, c.w);
       g.s[2 * h] = make_float2(s.x, s.y);
       g.s[2 * h + 1] = make_float2(s.z, s.w);
-      g.n[2 * h] = make_float2(-s.x, -s.y);
-      g.n[2 * h + 1] = make_float2(-s.z, -s.w);
     }
   }
 }
@@ -256,11 +260,9 @@ __device__ __forceinline__ void warp_angles(const uint64_t* s_turns, int pos, co
     if (p & 1) {
       g.c[p / 2].y = c;
       g.s[p / 2].y = s;
-      g.n[p / 2].y = -s;
     } else {
       g.c[p / 2].x = c;
       g.s[p / 2].x = s;
-      g.n[p / 2].x = -s;
     }
   }
 }
@@ -301,14 +303,15 @@ __device__ __forceinline__ bool locate(const NormRopeArgs& a, int b, int pos, bo
 // A warp takes a token (or, with few tokens, one of `slices` shares of its rows): nothing is shared between warps, no barrier.  Its
 // 32 / TPR row groups walk the query heads, the k heads and the v heads side by side, kR rows each per step (two independent chains
 // of reduction and arithmetic).  A thread brings its own pieces of the next steps into shared memory with asynchronous copies.  The
-// token's angles stay in registers for all rows, the weights too unless every head has its own.
+// token's angles stay in registers for all rows, the weights too unless every head has its own.  kOnlyQ: beside the blocks of an 8-bit cache, where
+// these rows are all there are and knowing so saves the registers that the kernel would spill.
 struct Cursor {  // of one row group: its rows of a step
   int s, row, n;
   int kind;            // 0 q, 1 k, 2 v
   int64_t off, step;   // bytes from the kind's base: of the first row, from row to row
 };
 
-template <int TPR, bool BF16, bool kNeox, int kFmt, int kT, int kR>
+template <int TPR, bool BF16, bool kNeox, int kFmt, int kT, int kR, bool kOnlyQ>
 __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, unsigned slices, int n_k, int n_v, const uint64_t* s_turns, uint4* s_rows) {
   constexpr int kSide = 32 / TPR;  // row groups of a warp
   constexpr int kSt = ring_stages(kR);
@@ -331,7 +334,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   const uint8_t* v_base = reinterpret_cast<const uint8_t*>(a.v) + kv_off;
 
   auto enter = [&](Cursor& c) {  // the kind that step c.s belongs to
-    c.kind = c.s < q_steps ? 0 : c.s < q_steps + k_steps ? 1 : 2;
+    c.kind = kOnlyQ || c.s < q_steps ? 0 : c.s < q_steps + k_steps ? 1 : 2;
     c.row = (c.s - (c.kind == 0 ? 0 : c.kind == 1 ? q_steps : q_steps + k_steps)) * kR * kSide + group;
     c.n = c.kind == 0 ? n_q : c.kind == 1 ? n_k : n_v;
     const int64_t stride = 2 * (c.kind == 0 ? a.q_stride[2] : a.kv_stride[2]);
@@ -342,7 +345,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
     ++c.s;
     c.row += kR * kSide;
     c.off += kR * c.step;
-    if (c.s == q_steps || c.s == q_steps + k_steps) enter(c);
+    if (!kOnlyQ && (c.s == q_steps || c.s == q_steps + k_steps)) enter(c);
   };
   Cursor in;  // the step to be fetched next
   in.s = s0;
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) norm_rope_rows_kernel(const No
   grid_launch_dependents();
   copy_turns<kRowThreads>(a, s_turns);
   grid_dependency_wait();
-  rows_role<TPR, BF16, kNeox, kFmt, kRowThreads, kR>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
+  rows_role<TPR, BF16, kNeox, kFmt, kRowThreads, kR, false>(a, blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices),
                                                  a.k != nullptr ? a.n_kv_heads : 0, a.v != nullptr ? a.n_kv_heads : 0, s_turns, s_rows);
 }
 
@@ -604,7 +607,6 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
         const float2 cs = angle_of(s_turns, base + row_a, p < 4 ? ch.i0 + p : ch.i1 + p - 4);
         (p & 1 ? first.c[p / 2].y : first.c[p / 2].x) = cs.x;
         (p & 1 ? first.s[p / 2].y : first.s[p / 2].x) = cs.y;
-        (p & 1 ? first.n[p / 2].y : first.n[p / 2].x) = -cs.y;
       }
     }
   }
@@ -640,9 +642,8 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 c = first.c[i];
-            angles.c[i] = __ffma2_rn(first.s[i], d.n[i], __fmul2_rn(c, d.c[i]));
+            angles.c[i] = minus_product(first.s[i], d.s[i], __fmul2_rn(c, d.c[i]));
             angles.s[i] = __ffma2_rn(first.s[i], d.c[i], __fmul2_rn(c, d.s[i]));
-            angles.n[i] = make_float2(-angles.s[i].x, -angles.s[i].y);
           }
         }
         float x[16];
@@ -720,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
     if (before & 1) block_role<TPR, BF16, kNeox, kFmt, false, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
     else block_role<TPR, BF16, kNeox, kFmt, true, kRows>(a, i / slices, i % slices, slices, s_turns, s_dyn, s_max);
   } else {
-    rows_role<TPR, BF16, kNeox, 0, kThreads, 2>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
+    rows_role<TPR, BF16, kNeox, 0, kThreads, 2, true>(a, (blockIdx.x - before) * (kThreads / 32) + threadIdx.x / 32, static_cast<unsigned>(a.slices), 0, 0,
                                              s_turns, reinterpret_cast<uint4*>(s_dyn));
   }
 }
