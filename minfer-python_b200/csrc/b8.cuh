@@ -80,7 +80,37 @@ __device__ __forceinline__ uint32_t int8_to_half2(uint32_t src) {
   return *reinterpret_cast<const uint32_t*>(&q);
 }
 
-// eight values -> eight codes; r = 1 / s.  Values of magnitude 127.5 s and above do not occur with int8: the scale follows the largest.
+// Whether a product with 1 / scale may miss the nearest e4m3 code: it is exact for powers of two, but a block that another program began may
+// have any scale (largest / 448, say), and keeps it until it has to grow.
+template <int kFmt>
+__device__ __forceinline__ bool b8_wants_quotient(float s) { return kFmt == kE4M3 && (__float_as_uint(s) & 0x7FFFFFu) != 0; }
+
+// x / s rounded to fp32, but to the odd one of its two neighbours where it is not exact: on the same side of every border between two codes as the
+// exact quotient, as a border has few bits.  The nearest fp32 cannot pass a border, only fall on one; the remainder's sign says which side is right.
+__device__ __forceinline__ float odd_quotient(float x, float s) {
+  if (s < 8.67361737988403547e-19f) {  // 2^-60: the remainder's last bit may lie below the smallest fp32
+    x *= 18446744073709551616.f;       // 2^64; finite values are no larger than 448 s
+    s *= 18446744073709551616.f;
+  }
+  const float q = __fdiv_rn(x, s);
+  const uint32_t bits = __float_as_uint(q);
+  if (!(fabsf(q) >= 2.44140625e-4f && fabsf(q) < 512.f) || (bits & 1u) != 0) return q;  // (2^-12: no borders below that)
+  const float rem = fmaf(-q, s, x);
+  return rem == 0.f ? q : __uint_as_float(bits + ((rem < 0.f) == (q < 0.f) ? 1u : 0xFFFFFFFFu));
+}
+
+// The e4m3 codes nearest to eight values, by the quotient
+__device__ __forceinline__ uint2 e4m3_code8(const float4& a, const float4& b, float s) {
+  return make_uint2(e4m3_pair(odd_quotient(a.x, s), odd_quotient(a.y, s)) | (e4m3_pair(odd_quotient(a.z, s), odd_quotient(a.w, s)) << 16),
+                    e4m3_pair(odd_quotient(b.x, s), odd_quotient(b.y, s)) | (e4m3_pair(odd_quotient(b.z, s), odd_quotient(b.w, s)) << 16));
+}
+// The same of values in x[0] and x[step]: in memory, out of the way of the kernel's registers
+static __device__ __noinline__ void e4m3_code_at(uint8_t* codes, const float4* x, int step, float s) {
+  *reinterpret_cast<uint2*>(codes) = e4m3_code8(x[0], x[step], s);
+}
+
+// eight values -> eight codes; r = 1 / s.  e4m3: for scales that are powers of two (b8_wants_quotient).
+// Values of magnitude 127.5 s and above do not occur with int8: the scale follows the largest.
 template <int kFmt>
 __device__ __forceinline__ uint2 b8_code8(const float* x, float s, float r) {
   uint32_t w[2];
@@ -140,12 +170,6 @@ __device__ __forceinline__ uint2 b8_recode8(uint2 c, float s0, float s1, float r
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= s0;
   return b8_code8<kFmt>(x, s1, r1);
-}
-
-// the same in memory, for rows that only now and then have to be coded again
-template <int kFmt>
-__device__ __noinline__ void b8_recode_at(uint2* p, float s0, float s1, float r1) {
-  *p = b8_recode8<kFmt>(*p, s0, s1, r1);
 }
 
 // rows [0, n) of a block (row_chunks 16-byte chunks each), coded again by `lanes` threads

@@ -384,7 +384,7 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
   int stage = 0;
   for (; at.s < s1; advance(at)) {
     cp_async_wait<kSt - 2>();
-    const uint4* sp = s_rows + stage * (2 * kR) * kT + tid;
+    uint4* sp = s_rows + stage * (2 * kR) * kT + tid;
     const bool both = kR == 2 && at.row - group + kSide < at.n;  // rows for the second half of the step
     uint4 raw[kR][2];
 #pragma unroll
@@ -482,6 +482,15 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
           uint8_t* dst = blk_rows + static_cast<int64_t>(begun) * a.cache_stride[2];
           *reinterpret_cast<uint2*>(dst + 8 * ch.c0) = b8_code8<kFmt>(x[u], o1, r1);
           *reinterpret_cast<uint2*>(dst + 8 * ch.c1) = b8_code8<kFmt>(x[u] + 8, o1, r1);
+          if (b8_wants_quotient<kFmt>(o1)) {  // (the thread's pieces of this step have been read: the values pass through their place)
+            float4* f = reinterpret_cast<float4*>(sp);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              f[0] = make_float4(x[u][8 * i], x[u][8 * i + 1], x[u][8 * i + 2], x[u][8 * i + 3]);
+              f[kT] = make_float4(x[u][8 * i + 4], x[u][8 * i + 5], x[u][8 * i + 6], x[u][8 * i + 7]);
+              e4m3_code_at(dst + 8 * (i ? ch.c1 : ch.c0), f, kT, o1);
+            }
+          }
         }
         __syncwarp();  // every lane of the row has read the scale
         if (row_ok && t == 0 && (begun == 0 || o1 != o0)) *sc = o1;  // (a block that begins here held anything)
@@ -539,6 +548,32 @@ __device__ __forceinline__ float raw_amax(const uint4& p, const uint4& q) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
     return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
+// What a thread's rows of a block that was begun may want besides, in one call out of the way of the registers: rows that were there (`old`, a bit each)
+// are coded again under a scale that grew, s0 -> s1; new ones are coded by the quotient where s1 is no power of two.  k's values still wait in shared
+// memory, v's are read again.
+template <bool BF16, int kFmt, bool kIsK>
+__device__ __noinline__ void rows_of_begun_block(uint8_t* dst, int64_t dst_step, const float4* val, const uint8_t* src, int64_t src_step, int c0, int c1, unsigned fresh,
+                                                 unsigned old, float s0, float s1) {
+  const float r1 = b8_inverse(s1);
+#pragma unroll 1
+  for (int i = 0; i < 2 * kMaxRows; ++i) {  // both chunks of every row
+    const int r = i >> 1, c = (i & 1) ? c1 : c0;
+    uint2* d = reinterpret_cast<uint2*>(dst + r * dst_step + 8 * c);
+    if ((old >> r) & 1u) {
+      *d = b8_recode8<kFmt>(*d, s0, s1, r1);
+    } else if (b8_wants_quotient<kFmt>(s1) && ((fresh >> r) & 1u)) {
+      float x[8];
+      if constexpr (kIsK) {
+        *reinterpret_cast<float4*>(x) = val[2 * i * kThreads];
+        *reinterpret_cast<float4*>(x + 4) = val[(2 * i + 1) * kThreads];
+      } else {
+        unpack8<BF16>(*reinterpret_cast<const uint4*>(src + r * src_step + 16 * c), x);
+      }
+      *d = e4m3_code8(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), s1);
+    }
   }
 }
 
@@ -694,12 +729,18 @@ __device__ __forceinline__ void block_role(const NormRopeArgs& a, unsigned unit,
         }
         *d0 = b8_code8<kFmt>(x, s1, r1);
         *d1 = b8_code8<kFmt>(x + 8, s1, r1);
-      } else if (head_ok && ch.live && row_a + r * row_step < lo && s1 != s0) {  // rows that were there, under a scale that grew
-        b8_recode_at<kFmt>(d0, s0, s1, r1);
-        b8_recode_at<kFmt>(d1, s0, s1, r1);
       }
     }
     if (!kIsK) cp_async_commit();
+    if (lo != 0 && (s1 != s0 || b8_wants_quotient<kFmt>(s1)) && head_ok && ch.live) {
+      unsigned fresh = 0, old = 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        if (is_new(r)) fresh |= 1u << r;
+        else if (row_a + r * row_step < lo && s1 != s0) old |= 1u << r;
+      }
+      rows_of_begun_block<BF16, kFmt, kIsK>(dst, dst_step, s_val, src + 2 * static_cast<int64_t>(h) * a.kv_stride[2], src_step, ch.c0, ch.c1, fresh, old, s0, s1);
+    }
     // one lane of the head's group
     if (head_ok && t == 0 && row_a == 0 && (lo == 0 || s1 != s0)) scales[static_cast<int64_t>(h) * a.scale_stride[1]] = s1;
   }

@@ -3,6 +3,8 @@ import pytest
 import torch
 
 from _b8 import Cache
+from oracle import oracle as O
+from test_b8_gpu import append, check_append
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +26,42 @@ def test_read_back_of_negative_lengths_touches_nothing(kerns, page):
         want = torch.full((B, H, c.rows + 64, D), 7.0, dtype=torch.float16)
         want[3, :, :5] = c.values(i)[3, :, :5].half()
         assert torch.equal(got[i], want), i
+
+
+def values_near_borders(dtype, scale, n):
+    """The n finite values of the type, of those that a block with this e4m3 scale takes without growing, whose quotient lies nearest to a border between two codes
+    (ties among them), half of them negative; shuffled."""
+    x = torch.arange(1 << 15, dtype=torch.int32).to(torch.int16).view(dtype).double()
+    m, e = torch.frexp(torch.tensor(float(scale), dtype=torch.float64))
+    x = x[torch.isfinite(x) & (x > scale * 2.0 ** -11) & (x <= 448 * torch.ldexp(torch.ones((), dtype=torch.float64), e - 1))]
+    y = x / scale
+    step = torch.exp2(torch.floor(torch.log2(y.clamp_min(2.0 ** -6))) - 3)
+    order = ((y / step - torch.floor(y / step) - 0.5).abs() * step / y).argsort()
+    x = x[order[:n]].repeat(-(-n // min(n, len(x))))[:n]
+    g = torch.Generator().manual_seed(n)
+    return (x * (1 - 2 * torch.randint(0, 2, (n,), generator=g)))[torch.randperm(n, generator=g)].to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [7.0, 49 / 448, 0.3, 1.9, 3 * 2.0 ** -10, 1.25 * 2.0 ** -66])
+@pytest.mark.parametrize("L,D,block,page", [(1, 128, 16, 0), (1, 64, 64, 64), (5, 64, 16, 48), (100, 128, 128, 0), (40, 128, 64, 128), (60, 64, 128, 0)])
+def test_e4m3_codes_under_scales_of_other_writers(kerns, dtype, scale, L, D, block, page):
+    """A block that another program began keeps its scale while the new rows need no larger one, whatever number it is: their codes are the nearest
+    ones, ties to even, of the exact quotient, as under a power of two."""
+    if dtype is torch.float16 and scale < 1e-10:
+        pytest.skip("float16 has no values there")
+    B, H = 2, 4
+    c = Cache("e4m3", B, H, 256, D, block, page, seed=12)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    for i in range(2):
+        c.scale[i][:] = scale
+    start = torch.tensor([1, block - 2], dtype=torch.int32)            # the second sequence's call goes on into blocks of its own
+    x = values_near_borders(dtype, scale, 2 * B * L * H * D).view(2, B, L, H, D)
+    k, v = x[0], x[1]
+    t = c.to_gpu()
+    append(kerns, c, t, 0, 0, k.cuda(), k.cuda(), v.cuda(), start)
+    torch.cuda.synchronize()
+    kept = c.scale[0].clone()
+    check_append(c, t, k.double(), start, 0, True, "k")
+    check_append(c, t, v.double(), start, 1, True, "v")
+    assert torch.equal(c.scale[0][0, :, 0], kept[0, :, 0]) and torch.equal(c.scale[0][1, :, 0], kept[1, :, 0]), "the scale was to stay"
