@@ -858,7 +858,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
     return tpr == 4 ? MINFER_NR_STYLE(launch_rows, 4, kInt8, a, nb, stream) : MINFER_NR_STYLE(launch_rows, 8, kInt8, a, nb, stream);
   }
   const int blk = 1 << a.log_block;
-  a.n_touch = (a.seq + blk - 2) / blk + 1;
+  a.n_touch = static_cast<int>((static_cast<int64_t>(a.seq) + blk - 2) / blk + 1);  // (a call may name nearly 2^31 tokens, of an expanded k and v)
   const long long units = static_cast<long long>(a.batch) * a.n_touch;
   const int abreast = (tpr << a.log_block) < kThreads ? kThreads / (tpr << a.log_block) : 1;  // heads side by side
   const int head_groups = (a.n_kv_heads + abreast - 1) / abreast;

@@ -65,3 +65,31 @@ def test_e4m3_codes_under_scales_of_other_writers(kerns, dtype, scale, L, D, blo
     check_append(c, t, k.double(), start, 0, True, "k")
     check_append(c, t, v.double(), start, 1, True, "v")
     assert torch.equal(c.scale[0][0, :, 0], kept[0, :, 0]) and torch.equal(c.scale[0][1, :, 0], kept[1, :, 0]), "the scale was to stay"
+
+
+def test_append_of_nearly_two_to_the_31_tokens(kerns):
+    """Positions behind the cache are dropped and reported, so the C entry takes a call of 2^31 - 100 tokens whose k and v are one row, expanded; the number of
+    blocks that such a call touches passes 32 bits on the way."""
+    import ctypes
+
+    from minfer.kernels.torch_ext import _lib
+    D, H, rows, block = 64, 2, 64, 128
+    c = Cache("e4m3", 1, H, rows, D, block, seed=4)
+    t = c.to_gpu()
+    x = torch.randn(2, H, D, generator=torch.Generator().manual_seed(2)).half()
+    xd, start, status = x.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    p = _lib.NormRopeParams()
+    p.k, p.v, p.start, p.status = xd[0].data_ptr(), xd[1].data_ptr(), start.data_ptr(), status.data_ptr()
+    p.k_cache, p.v_cache, p.k_scale, p.v_scale = (y.data_ptr() for y in t)
+    p.kv_stride[2] = D
+    for i in range(3):
+        p.cache_stride[i] = t[0].stride(i)
+    p.scale_stride[0], p.scale_stride[1] = t[2].stride(0), t[2].stride(1)
+    p.batch, p.seq, p.n_kv_heads, p.head_dim, p.max_len = 1, 2 ** 31 - 100, H, D, rows
+    p.freq_base, p.dtype, p.cache_format, p.block_size = 10000.0, _lib.F16, _lib.KV_E4M3, block
+    rc = _lib.lib.minfer_attn_norm_rope_append(ctypes.byref(p), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert status.tolist() == [102, 0, rows, rows]
+    for i in range(2):
+        check_append(c, t, x[i].double().expand(1, rows, H, D), torch.zeros(1, dtype=torch.int32), i, True, str(i))
