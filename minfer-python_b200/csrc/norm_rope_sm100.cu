@@ -456,10 +456,10 @@ __device__ __forceinline__ void rows_role(const NormRopeArgs& a, unsigned item, 
       }
     } else if constexpr (kFmt != 0) {
       if (!cache_ok) continue;
+      static_assert(kR == 1, "an 8-bit cache takes its rows one by one");
       const int begun = crow & ((1 << a.log_block) - 1);  // rows of the block that are there
 #pragma unroll
       for (int u = 0; u < kR; ++u) {
-        if (u == 1 && !both) break;
         const int h = at.row + u * kSide;
         const bool row_ok = h < at.n;
         float* sc = (kind == 1 ? a.k_scale : a.v_scale) + static_cast<int64_t>(outer) * a.scale_stride[0] + static_cast<int64_t>(h) * a.scale_stride[1] + (crow >> a.log_block);
