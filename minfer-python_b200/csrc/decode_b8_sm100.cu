@@ -121,7 +121,7 @@ __device__ __forceinline__ void start_pair(const DecodeB8Args& a, int b, int kvh
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
       top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
       // the largest becomes 2^14 .. 2^15; exponents kept so that neither factor leaves fp32's range
-      const int e = max(-110, min(110, 127 + 14 - static_cast<int>(top >> 7)));
+      const int e = max(-113, min(110, 127 + 14 - static_cast<int>(top >> 7)));  // (-113: the largest finite exponent)
       const float f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
       back = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll

@@ -93,3 +93,23 @@ def test_append_of_nearly_two_to_the_31_tokens(kerns):
     assert status.tolist() == [102, 0, rows, rows]
     for i in range(2):
         check_append(c, t, x[i].double().expand(1, rows, H, D), torch.zeros(1, dtype=torch.int32), i, True, str(i))
+
+
+def test_decode_of_the_largest_queries(kerns):
+    """bfloat16 queries up to the type's last binade, 2^127 and more: finite scores, so a result as for any other query.  Scores differ by 2^119 and more from key
+    to key: the output is the value of the key with the largest."""
+    D, H, rows = 64, 4, 40
+    c = Cache("e4m3", 1, 1, rows, D, 16, seed=21)
+    c.codes[0].zero_()
+    c.scale[0][:] = 2.0 ** -10
+    order = torch.randperm(rows, generator=torch.Generator().manual_seed(4))
+    ladder = torch.tensor([m * 2.0 ** e for e in range(3, 8) for m in (1, 1.125, 1.25, 1.375, 1.5, 1.625, 1.75, 1.875)], dtype=torch.float64)
+    c.codes[0][0, 0, order, 5] = ladder[:rows]
+    q = torch.zeros(1, H, 1, D)
+    q[0, :, 0, 5] = torch.tensor([2.0 ** 125, 2.0 ** 126, -(2.0 ** 127), 2.0 ** 127 * 1.9921875])
+    q = q.bfloat16()
+    out = torch.zeros(1, H, 1, D, dtype=torch.bfloat16, device="cuda")
+    kerns.flash_attn_decode_b8(q.cuda(), *c.to_gpu(), 16, torch.tensor([rows], dtype=torch.int32, device="cuda"), out)
+    score = q[0, :, 0, 5, None].double() * c.values(0)[0, 0, :, 5] / 8
+    assert score.abs().max() < torch.finfo(torch.float32).max
+    assert torch.equal(out.cpu()[0, :, 0], c.values(1)[0, 0, score.argmax(1)].bfloat16())
