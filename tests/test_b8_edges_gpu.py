@@ -95,6 +95,48 @@ def test_append_of_nearly_two_to_the_31_tokens(kerns):
         check_append(c, t, x[i].double().expand(1, rows, H, D), torch.zeros(1, dtype=torch.int32), i, True, str(i))
 
 
+@pytest.mark.parametrize("dtype,style", [(torch.bfloat16, 1), (torch.float16, 0)])
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 32), (128, 64), (64, 128), (128, 128)])
+def test_tokens_in_one_call_or_one_by_one(kerns, dtype, style, D, block):
+    """e4m3: the same scales, and v's codes differ only where a value lies below the smallest normal code of the final scale.  So do k's where a thread
+    works on one row of a block (blocks of 4096 values and fewer); else a row's angle may be the sum of two, which moves k by 2^-18 of its row's
+    largest value at most in either form, and codes and scales where a border is as near as twice that."""
+    B, L, Hq, Hkv, rot = 2, 150, 4, 2, D
+    g = torch.Generator().manual_seed(D + block)
+    q, k, v = ((torch.randn(B, L, h, D, generator=g) * torch.exp(torch.randn(B, L, 1, 1, generator=g))).to(dtype) for h in (Hq, Hkv, Hkv))
+    qw, kw = (1 + 0.2 * torch.randn(D, generator=g), 1 + 0.2 * torch.randn(D, generator=g))
+    caches, tensors, qs = [], [], []
+    for whole in (True, False):
+        c = Cache("e4m3", B, Hkv, 256, D, block, seed=1)
+        t = c.to_gpu()
+        qd, kd, vd = q.cuda(), k.cuda(), v.cuda()
+        for p in ([(0, L)] if whole else [(i, i + 1) for i in range(L)]):
+            append(kerns, c, t, rot, style, qd[:, p[0]:p[1]], kd[:, p[0]:p[1]], vd[:, p[0]:p[1]], torch.full((B,), p[0], dtype=torch.int32), qw, kw)
+        torch.cuda.synchronize()
+        caches.append(c)
+        tensors.append(t)
+        qs.append(qd.cpu())
+    assert torch.equal(*qs)                                            # q's angles are formed in one way
+    y = O.norm_rope(k, kw, rot, 500000.0, style, [0] * B, 1e-6).transpose(1, 2), v.double().transpose(1, 2)
+    for i in range(2):
+        (ca, sa), (cb, sb) = (c.back(t[i], t[2 + i]) for c, t in zip(caches, tensors))
+        near = y[i].abs().amax(-1, keepdim=True) * (2.0 ** -17 if i == 0 and block * D > 4096 else 0.0)
+        blocks = -(-L // block)
+        for j in range(blocks):
+            top = y[i][:, :, j * block:(j + 1) * block].abs().amax((-1, -2))
+            low = torch.minimum(sa[:, :, j], sb[:, :, j])
+            assert ((sa[:, :, j] == sb[:, :, j]) | ((top - 448 * low).abs() <= near.amax())).all(), (i, j)
+        s = torch.maximum(sa, sb).repeat_interleave(block, -1)[:, :, :L, None]
+        a, b = (c[:, :, :L] * w.repeat_interleave(block, -1)[:, :, :L, None] for c, w in ((ca, sa), (cb, sb)))
+        z = y[i] / s
+        step = torch.exp2(torch.floor(torch.log2(z.abs().clamp_min(2.0 ** -6))) - 3)
+        border = ((z / step - torch.floor(z / step) - 0.5).abs() * step * s)
+        fine = (a == b) | (z.abs() < 2.0 ** -6) | (border <= near)
+        assert fine.all(), (i, int((~fine).sum()))
+        assert (z.abs() < 2.0 ** -6).double().mean() < 0.2             # (the rule above is about a few)
+        assert torch.equal(ca[:, :, L:], cb[:, :, L:])
+
+
 def test_decode_of_the_largest_queries(kerns):
     """bfloat16 queries up to the type's last binade, 2^127 and more: finite scores, so a result as for any other query.  Scores differ by 2^119 and more from key
     to key: the output is the value of the key with the largest."""
