@@ -327,7 +327,7 @@ int minfer_attn_rope_append(const MinferRopeParams* params, void* stream);
  * KV cache held in 8 bits ("b8"): codes [batch, n_kv_heads, max_len, head_dim], or a pool of pages
  * [n_pages, n_kv_heads, page_size, head_dim] behind a block table, and one fp32 scale for each block of block_size
  * consecutive rows of one head: [batch, n_kv_heads, ceil(max_len / block_size)], or [n_pages, n_kv_heads, page_size / block_size].
- * A cached value is code * scale.  Codes are e4m3 (no infinities; 448 is the largest) or int8 (-127 .. 127);
+ * A cached value is code * scale (where it is formed, in fp32).  Codes are e4m3 (no infinities; 448 is the largest) or int8 (-127 .. 127);
  * block_size is 16, 32, 64 or 128 and divides page_size; head_dim is 64 or 128.  The reference has no such cache.
  *
  * Code strides are in bytes (= elements), innermost 1, the others multiples of 16; bases 16-byte aligned.  Scale strides are in
@@ -353,6 +353,7 @@ int minfer_attn_rope_append(const MinferRopeParams* params, void* stream);
  *   - A block whose first row is written by this call takes its scale afresh.  A block that holds rows already (start[b] is not a
  *     multiple of block_size) keeps them: its scale grows when the new rows need it, and then the rows before
  *     start[b] are coded again from the values that they stood for.  It never shrinks.  Rows behind the last new one are not touched.
+ *     A block that another program began may have any scale; it keeps it, and codes are the nearest under it, until the rule above asks for more.
  * Positions outside [0, max_len) are not written (q is still rewritten) and reported through `status`, as are entries of the
  * block table outside [0, n_pages).  The caller sees to it that no two sequences append to the same page.
  * What is written has a stride in every dimension of more than one entry; q is neither k nor v, k_cache (k_scale) not v_cache (v_scale).
@@ -441,7 +442,7 @@ int minfer_attn_decode_b8(const MinferAttnDecodeB8Params* params, void* stream);
 size_t minfer_attn_decode_b8_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv_heads, int32_t max_len, int32_t head_dim);
 
 /*
- * Rows of a b8 cache as 16-bit values (code * scale, rounded once): row j of sequence b to row j of k_out / v_out
+ * Rows of a b8 cache as 16-bit values (code * scale in fp32, rounded to the type): row j of sequence b to row j of k_out / v_out
  * [batch, n_kv_heads, out_rows, head_dim] for j < min(lens[b], max_len, out_rows); the other rows of the outputs are not touched.  For the
  * attention of a prompt behind a cached prefix (minfer_attn_prefill reads 16-bit keys and values).
  * k_out and v_out are two buffers; min(max_len, out_rows) is at most 2^31 - 129.

@@ -5,6 +5,7 @@
 //         again under a larger scale keep their values (unless they fall below the smallest normal code, 2^-6).
 //   int8  scale = fp32(largest magnitude / 127): a fixed step, where a power of two would cost up to a bit.
 //   code  = the one nearest to x / scale, ties to even.  Infinite values saturate; NaN stays NaN in e4m3 and becomes 0 in int8.
+// Rows are coded again from code * scale in fp32.
 // A block of zeros has scale 0 and codes 0; no other scale is below 2^-126.
 #pragma once
 

@@ -10,8 +10,8 @@
 //
 // A tile lies inside one block of tokens, so its two scales are uniform and neither costs a multiplication per value: ks goes
 // into the factor that the scores take anyway, vs into the weights.  Codes of both kinds are exact in fp16, so all products are
-// fp16 MMAs on unscaled codes; bfloat16 queries are brought into fp16's range by a power of two per head (exact but for
-// elements below 2^-39 of the head's largest).
+// fp16 MMAs on unscaled codes; bfloat16 queries are brought into fp16's range by a power of two per head, under which the largest lies in 2^14 .. 2^15: exact down
+// to about 2^-31 of it, and below that off by at most half of fp16's last step, 2^-25, which is 2^-39 of the largest.
 //
 // Weights: w_j = 2^(t_j - m) vs_j is what is rounded to fp16.  m follows max_j(t_j + ceil(log2 vs_j)) - 14, not max t_j, so that
 // whatever the scales are the largest weight lies in (2^13, 2^14]: fp16 has full precision down to 2^-14, so weights keep theirs down to
@@ -23,8 +23,9 @@
 // 16-byte reads - K: chunks 2 tq and 2 tq + 1 of key g0; V: chunk g0 of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 - meet no bank twice.
 // A lane takes consecutive dimensions: for K that permutes the summands of an MMA, for V the rows of the output.
 //
-// Measured (32 / 8 heads, D=128, back to back): 64 sequences of 512-8192 keys, e4m3, 91.9 us, 6.2 TB/s, 0.96 of what a copy reaches; ragged
-// int8 pages of 64 keys, 24 sequences of up to 10001 with 48 heads, 59.9 us, 0.68 (the same in one piece 52.8).
+// Measured (32 / 8 heads, D=128, back to back in a graph): 64 sequences of 512-8192 keys, e4m3, 92.7 us, 6.2 TB/s, 0.96 of what a copy reaches (102 us, 0.87, as a
+// call among other work).  24 ragged sequences of up to 10001, 48 / 8 heads, in one piece / pages of 64 / of 256 keys: e4m3 49.6 / 54.2 / 53.8 us, int8 53.3 / 60.6 /
+// 60.4, 0.67 of a copy: a block's look-ups per tile (a division, three products) are 14 % more instructions at the same issue rate (55 % of cycles, ALU 48 %).
 #include "b8.cuh"
 #include "decode_common.cuh"
 

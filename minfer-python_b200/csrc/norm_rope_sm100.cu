@@ -15,9 +15,9 @@
 // A row (one head of one token) belongs to TPR = 4, 8 or 16 lanes with two 16-byte chunks each; in the two-halves form they are a chunk and
 // its partner, so a rotated pair never leaves its thread.
 //
-// Measured (32 / 8 heads, D=128, 4 x 4096 tokens, back to back): 16-bit cache 63.9 us, 6.3 TB/s, 0.98 of what a copy reaches; 8-bit cache (e4m3,
-// blocks of 128) 76.4 us, 4.8 TB/s, bound by issue slots (55 % busy) and latency at 16 warps per SM; single tokens of 64 sequences 3.0 and
-// 3.1 us, launch and latency.
+// Measured (32 / 8 heads, D=128, 4 x 4096 tokens, back to back): 16-bit cache 64.4 us, 6.3 TB/s, 0.97 of what a copy reaches; 8-bit cache (e4m3,
+// blocks of 128) 71.8 us, 5.1 TB/s, with norms 83 us, bound by issue slots (56 % busy) and latency at 16 warps per SM; single tokens of 64 sequences 3.1 and
+// 3.2-3.4 us, launch and latency.
 #include "../../include/minfer_attn.h"
 #include "attn_internal.h"
 #include "b8.cuh"
@@ -767,7 +767,8 @@ __global__ void __launch_bounds__(kThreads, 2) norm_rope_blocks_kernel(const Nor
   }
 }
 
-// frequencies in turns: base ^ (-2 i / rotary_dim) / (2 pi), modulo 1 (positions are whole numbers), as fractions of 2^64
+// Frequencies in turns: base ^ (-2 i / rotary_dim) / (2 pi), modulo 1 (positions are whole numbers), as fractions of 2^64.  A thread keeps those of its last base:
+// calls that change it (or rotary_dim) take 17 us more of host time each (64 pairs; 20.1 us per call instead of 3.0), which a captured graph does not.
 void fill_turns(NormRopeArgs& a, double freq_base) {
   thread_local double cached_base = 0.0;
   thread_local int cached_rot = -1;
@@ -863,7 +864,7 @@ cudaError_t launch_norm_rope(const NormRopeArgs& a_in, bool bf16, bool neox, int
   const int abreast = (tpr << a.log_block) < kThreads ? kThreads / (tpr << a.log_block) : 1;  // heads side by side
   const int head_groups = (a.n_kv_heads + abreast - 1) / abreast;
   // A unit's heads over several blocks while all units together are fewer than two per SM; fewer blocks share the angles better (us with this /
-  // twice as many: 8 x 512 tokens, D=64, blocks of 16: 15.1 / 17.4; 4 x 4096, D=128, blocks of 128: 74.7 / 73.4).
+  // twice as many: 8 x 512 tokens, D=64, blocks of 16: 16.1 / 18.4; 4 x 4096, D=128, blocks of 128: 71.7 / 69.9).
   long long kv_slices = 2 * 148 / units;
   if (kv_slices > head_groups) kv_slices = head_groups;
   if (kv_slices < 1) kv_slices = 1;

@@ -847,8 +847,8 @@ def flash_attn_decode_b8_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: 
 def kv_read_b8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block_size: int,
                lens: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor):
     """
-    rows [0, lens[b]) of a cache held in 8 bits (layout: rope_kv_append_b8) as 16-bit values, code * scale rounded once, into k_out and
-    v_out [B, Hkv, rows, D] (float16 or bfloat16); rows of the outputs behind lens[b] are left as they are.  For
+    rows [0, lens[b]) of a cache held in 8 bits (layout: rope_kv_append_b8) as 16-bit values, code * scale in float32 rounded to the type, into
+    k_out and v_out [B, Hkv, rows, D] (float16 or bfloat16); rows of the outputs behind lens[b] are left as they are.  For
     flash_attn_causal of a prompt behind a cached prefix.
     """
     if _direct is not None and not _is_compiling() and _direct.kv_read_b8(k_cache, v_cache, k_scale, v_scale, block_size, lens, k_out, v_out):
