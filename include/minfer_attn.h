@@ -328,7 +328,7 @@ int minfer_attn_rope_append(const MinferRopeParams* params, void* stream);
  * [n_pages, n_kv_heads, page_size, head_dim] behind a block table, and one fp32 scale for each block of block_size
  * consecutive rows of one head: [batch, n_kv_heads, ceil(max_len / block_size)], or [n_pages, n_kv_heads, page_size / block_size].
  * A cached value is code * scale (where it is formed, in fp32).  Codes are e4m3 (no infinities; 448 is the largest) or int8 (-127 .. 127);
- * block_size is 16, 32, 64 or 128 and divides page_size; head_dim is 64 or 128.  The reference has no such cache.
+ * scales are not negative; block_size is 16, 32, 64 or 128 and divides page_size; head_dim is 64 or 128.  The reference has no such cache.
  *
  * Code strides are in bytes (= elements), innermost 1, the others multiples of 16; bases 16-byte aligned.  Scale strides are in
  * elements for the two outer dimensions; a head's scales are adjacent.  k and v share all strides.

@@ -169,7 +169,10 @@ __device__ __forceinline__ uint2 b8_recode8(uint2 c, float s0, float s1, float r
   float x[8];
   b8_values8<kFmt>(c, x);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= s0;
+  for (int i = 0; i < 8; ++i) {
+    x[i] *= s0;
+    if constexpr (kFmt == kInt8) x[i] = fmaxf(x[i], -127.f * s1);  // (another program's code -128 may pass the largest magnitude of s1)
+  }
   return b8_code8<kFmt>(x, s1, r1);
 }
 

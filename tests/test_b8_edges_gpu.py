@@ -42,14 +42,12 @@ def values_near_borders(dtype, scale, n):
     return (x * (1 - 2 * torch.randint(0, 2, (n,), generator=g)))[torch.randperm(n, generator=g)].to(dtype)
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("scale", [7.0, 49 / 448, 0.3, 1.9, 3 * 2.0 ** -10, 1.25 * 2.0 ** -66])
+@pytest.mark.parametrize("dtype,scale", [(t, s) for t in (torch.float16, torch.bfloat16) for s in (7.0, 49 / 448, 0.3, 1.9, 3 * 2.0 ** -10)] +
+                                        [(torch.bfloat16, 1.25 * 2.0 ** -66)])
 @pytest.mark.parametrize("L,D,block,page", [(1, 128, 16, 0), (1, 64, 64, 64), (5, 64, 16, 48), (100, 128, 128, 0), (40, 128, 64, 128), (60, 64, 128, 0)])
 def test_e4m3_codes_under_scales_of_other_writers(kerns, dtype, scale, L, D, block, page):
     """A block that another program began keeps its scale while the new rows need no larger one, whatever number it is: their codes are the nearest
     ones, ties to even, of the exact quotient, as under a power of two."""
-    if dtype is torch.float16 and scale < 1e-10:
-        pytest.skip("float16 has no values there")
     B, H = 2, 4
     c = Cache("e4m3", B, H, 256, D, block, page, seed=12)
     scale = float(torch.tensor(scale, dtype=torch.float32))
@@ -155,3 +153,24 @@ def test_decode_of_the_largest_queries(kerns):
     score = q[0, :, 0, 5, None].double() * c.values(0)[0, 0, :, 5] / 8
     assert score.abs().max() < torch.finfo(torch.float32).max
     assert torch.equal(out.cpu()[0, :, 0], c.values(1)[0, 0, score.argmax(1)].bfloat16())
+
+
+@pytest.mark.parametrize("L", [1, 30])
+@pytest.mark.parametrize("page", [0, 64])
+def test_the_int8_code_of_minus_128_saturates_under_a_scale_that_grew_little(kerns, L, page):
+    """Another program's -128 is read as what it is; coded again under a scale up to 128 / 127 of the old one it lies beyond -127 steps, the last code there is."""
+    B, H, D, block = 1, 4, 64, 64
+    c = Cache("int8", B, H, 128, D, block, page, seed=9)
+    for i in range(2):
+        c.codes[i][:, :, :20] = torch.where(torch.arange(D) % 3 == 0, -128.0, c.codes[i][:, :, :20])
+        c.scale[i][:, :, 0] = 1.0
+    t = c.to_gpu()
+    x = torch.ones(B, L, H, D)
+    x[0, 0, :, 7] = torch.tensor([127.0625, 127.5, 128.0, 129.0])     # scales of 1.0005, 1.004, 1.0079 and 1.0157
+    x = x.half()
+    start = torch.tensor([20], dtype=torch.int32)
+    append(kerns, c, t, 0, 0, x.cuda(), x.cuda(), x.cuda(), start)
+    torch.cuda.synchronize()
+    for i in range(2):
+        check_append(c, t, x.double(), start, i, True, str(i))
+        assert c.codes[i].min() == -127.0
