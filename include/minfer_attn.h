@@ -403,7 +403,8 @@ int minfer_attn_norm_rope_append(const MinferNormRopeParams* params, void* strea
 /*
  * Decode attention (one query token per sequence) over a b8 cache; q, out, lens, softmax_scale, block_table and status as in
  * MinferAttnDecodeParams.  Rows at lens[b] and behind, and their scales, are never read.  lens[b] == 0 yields zeros; a NaN among
- * the visible values reaches the outputs that it enters.
+ * the visible values reaches the outputs that it enters.  v's scales are taken to be 0 or to lie in 2^-104 .. 2^36 (values up to 3e13): with others
+ * beside them small blocks may lose bits or their part of the softmax's sum.
  * workspace: minfer_attn_decode_b8_workspace_bytes() bytes, 16-byte aligned, any content; 0 for most shapes.  Without it
  * a shape that would use it takes another form (slower; the sums are split differently).
  */

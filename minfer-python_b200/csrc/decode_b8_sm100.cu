@@ -17,7 +17,8 @@
 // whatever the scales are the largest weight lies in (2^13, 2^14]: fp16 has full precision down to 2^-14, so weights keep theirs down to
 // 2^-28 of the largest, and a long tail of equal small weights is not rounded in one direction.  The row sum takes 2^(t_j - m)
 // in fp32, before the scale and before the rounding.  log2 vs_j counts as -90 or more: 2^104 times the number of keys fits
-// fp32, and a block of zeros (scale 0) has weights of 0.
+// fp32, and a block of zeros (scale 0) has weights of 0.  References of different blocks are then up to 90 + log2 of the largest scale apart, which fp32
+// holds to 126: from scales of v above 2^36 on (values of 3e13) the share that blocks of zeros have in the sum may be lost.
 //
 // Shared memory: rows of 128 bytes with the 16-byte chunks XORed by the row, pairs of rows of 64 bytes likewise by their line, so that a lane's
 // 16-byte reads - K: chunks 2 tq and 2 tq + 1 of key g0; V: chunk g0 of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9 - meet no bank twice.
